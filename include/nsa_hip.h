@@ -442,6 +442,24 @@ int nsa_decode_step_split_static(const void* q, const void* k_cache, const void*
                                  int pool_stride, int pool_pad, int top_n, int window, float scale, int gate_act,
                                  int dtype, int splits, nsa_stream_t stream);
 
+/* Dense decode attention: the one new token of every sequence attends ALL its cached tokens (window = 0) or the last
+ * `window` of them, the current one among them.  Cache layouts as above; block_table NULL = contiguous caches (ctx_cap
+ * used, a multiple of 64), else the paged pool of num_pages pages (max_pages used).  The compressed caches are not read.
+ *   q [batch][hq][dk]   out [batch][hq][dv]   lse (optional) float [batch][hq]: natural-log log-sum-exp of the scaled scores
+ * A sequence with ctx_lens[b] <= 0 yields out = 0 and lse = -inf; a length beyond the capacity counts as the capacity.
+ * What the cache holds behind a sequence's last token, or before its window, does not matter (not even NaN).  A table
+ * entry outside the pool is read as page 0.  Any GQA group size; (dk, dv) in (32,32), (64,64), (128,128), (192,128).
+ * The cached tokens of all sequences are cut into equal pieces on the device, from ctx_lens, so the grid and the
+ * workspace depend on the arguments alone and a captured call stays right while the sequences grow.  The result of a
+ * sequence depends on where it is cut, hence to rounding on the other lengths of the batch; equal calls give equal bits.
+ * workspace: nsa_dense_decode_workspace_bytes (0 for short capacities; ctx_cap = 64 * max_pages when paged; -1 for
+ * invalid sizes); calls that share it must not overlap.  No counterpart in the reference, which has no cache. */
+int64_t nsa_dense_decode_workspace_bytes(int batch, int hq, int hkv, int dk, int dv, int ctx_cap, int window, int dtype);
+int nsa_dense_decode_step(const void* q, const void* k_cache, const void* v_cache_t, const int32_t* block_table,
+                          int max_pages, int num_pages, const int32_t* ctx_lens, void* out, float* lse, int batch, int hq,
+                          int hkv, int dk, int dv, int ctx_cap, int window, float scale, int dtype, void* workspace,
+                          int64_t workspace_bytes, nsa_stream_t stream);
+
 /* Appends one token per sequence: k_new [batch][hkv][dk] -> row pos[b] of k_cache, v_new
  * [batch][hkv][dv] -> column pos[b] of v_cache_t, and, when pos[b]+1 completes a compression block,
  * the mean of the last `block` tokens as the next row / column of the compressed caches. */

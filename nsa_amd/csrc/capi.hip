@@ -1,6 +1,7 @@
 // extern "C" boundary of libnsa_hip.so: argument checks, error strings, dispatch to the launchers.
 #include <stdio.h>
 #include <stdarg.h>
+#include <string.h>
 
 #include "../../include/nsa_hip.h"
 #include "common.h"
@@ -796,6 +797,55 @@ int nsa_decode_step_paged(const void* q, const void* k_pool, const void* v_pool_
   return decode_common("decode_step_paged", q, k_pool, v_pool_t, block_table, max_pages, ck_cache, cv_cache_t, ctx_lens,
                        gates, out, indices, batch, hq, hkv, dk, dv, max_pages * 64, nc_cap, block, stride, sel_block,
                        pool_kernel, pool_stride, pool_pad, top_n, window, scale, gate_act, dtype, stream);
+}
+
+static nsa::DenseDecodeArgs dense_args(int batch, int hq, int hkv, int dk, int dv, int ctx_cap, int window, int dtype) {
+  nsa::DenseDecodeArgs a{};
+  a.batch = batch; a.hq = hq; a.hkv = hkv; a.dk = dk; a.dv = dv; a.ctx_cap = ctx_cap; a.window = window; a.dtype = dtype;
+  return a;
+}
+// by its bits: the library is compiled with the promise that no NaN occurs, which lets arithmetic tests fold away
+static bool finite_bits(float x) {
+  uint32_t u;
+  memcpy(&u, &x, sizeof(u));
+  return (u & 0x7f800000u) != 0x7f800000u;
+}
+static bool dense_sizes_ok(int batch, int hq, int hkv, int ctx_cap, int window) {
+  return batch > 0 && hq > 0 && hkv > 0 && hq % hkv == 0 && ctx_cap > 0 && ctx_cap % 64 == 0 && window >= 0 &&
+         (int64_t)batch * (ctx_cap / 64) <= 0x7fffffff;
+}
+
+int64_t nsa_dense_decode_workspace_bytes(int batch, int hq, int hkv, int dk, int dv, int ctx_cap, int window, int dtype) {
+  if (!dense_sizes_ok(batch, hq, hkv, ctx_cap, window) || dk <= 0 || dv <= 0 || !dtype_ok(dtype)) return -1;
+  return nsa::dense_decode_workspace_bytes(dense_args(batch, hq, hkv, dk, dv, ctx_cap, window, dtype));
+}
+
+int nsa_dense_decode_step(const void* q, const void* k_cache, const void* v_cache_t, const int32_t* block_table,
+                          int max_pages, int num_pages, const int32_t* ctx_lens, void* out, float* lse, int batch, int hq,
+                          int hkv, int dk, int dv, int ctx_cap, int window, float scale, int dtype, void* workspace,
+                          int64_t workspace_bytes, nsa_stream_t stream) {
+  if (!q || !k_cache || !v_cache_t || !ctx_lens || !out) return fail(NSA_ERR_INVALID, "dense_decode: null pointer");
+  if (!dtype_ok(dtype)) return fail(NSA_ERR_INVALID, "dense_decode: bad dtype");
+  if (block_table) {
+    if (max_pages <= 0 || num_pages <= 0) return fail(NSA_ERR_INVALID, "dense_decode: a block table needs max_pages and num_pages");
+    if (max_pages > 0x7fffffff / 64) return fail(NSA_ERR_INVALID, "dense_decode: max_pages too large");
+    ctx_cap = max_pages * 64;
+  }
+  if (!dense_sizes_ok(batch, hq, hkv, ctx_cap, window))
+    return fail(NSA_ERR_INVALID, "dense_decode: sizes must be positive, hq a multiple of hkv, ctx_cap of 64, window >= 0 and "
+                                 "batch * pages below 2^31");
+  if (!finite_bits(scale)) return fail(NSA_ERR_INVALID, "dense_decode: scale must be finite");
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache_t) || !aligned16(out))
+    return fail(NSA_ERR_INVALID, "dense_decode: pointers must be 16-byte aligned");
+  nsa::DenseDecodeArgs a = dense_args(batch, hq, hkv, dk, dv, ctx_cap, window, dtype);
+  a.q = q; a.k = k_cache; a.v = v_cache_t; a.block_table = block_table; a.ctx_lens = ctx_lens; a.out = out; a.lse = lse;
+  a.max_pages = max_pages; a.num_pages = num_pages; a.scale = scale;
+  const int64_t need = nsa::dense_decode_workspace_bytes(a);
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+    return fail(NSA_ERR_INVALID, "dense_decode: workspace missing, misaligned or smaller than nsa_dense_decode_workspace_bytes");
+  const int rc = nsa::launch_dense_decode(a, workspace, stream);
+  if (rc == -5) return fail(NSA_ERR_UNSUPPORTED, "dense_decode: more than 2^31-1 workgroups");
+  return finish(rc, "dense_decode");
 }
 
 int nsa_decode_append(const void* k_new, const void* v_new, void* k_cache, void* v_cache_t, void* ck_cache,

@@ -141,6 +141,19 @@ struct DecodeArgs {
   int kv_rep = 1;
 };
 
+// Dense decode attention over all cached tokens (or the last `window`): block_table null = contiguous caches.
+struct DenseDecodeArgs {
+  const void* q; const void* k; const void* v; const int32_t* block_table; const int32_t* ctx_lens;
+  void* out; float* lse;                                   // lse may be null
+  int batch, hq, hkv, dk, dv, ctx_cap, max_pages, num_pages, window;
+  float scale; int dtype;
+  int units; float* part; float* part_ml;                  // filled in by the launch
+};
+struct DensePlan { int tiles, blocks, units, rows; long slots; bool split; };
+DensePlan dense_decode_plan(const DenseDecodeArgs& a);
+long dense_decode_workspace_bytes(const DenseDecodeArgs& a);
+int launch_dense_decode(DenseDecodeArgs a, void* workspace, hipStream_t st);
+
 // Split of a projection GEMM's packed rows [q | k | v | gate logits] into the attention operands with
 // the rotary embedding applied to q and k (pack == 0), or the reverse gather of their gradients with
 // the inverse rotation (pack == 1).  Column offsets and ld in elements, multiples of 8 except g_off.

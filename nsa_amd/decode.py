@@ -11,7 +11,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .ops import _dtype_code, _ptr, _stream
+from .ops import _dense, _dtype_code, _need_cuda, _on_device_of, _ptr, _stream
 
 
 def _round_up(x: int, m: int) -> int:
@@ -339,6 +339,52 @@ def nsa_decode_step(q: torch.Tensor, cache, gates: Optional[torch.Tensor] = None
         _dtype_code(q), _stream())
     _lib.check(rc, "nsa_decode_step")
     return (out, idx) if return_indices else out
+
+
+@torch.no_grad()
+def dense_decode_step(q: torch.Tensor, cache, scale: Optional[float] = None, sliding_window: int = 0,
+                      return_lse: bool = False, out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None):
+    """Full attention of one new token per sequence: q [B,Hq,Dk] attends every cached token of its sequence, or the last
+    `sliding_window` of them when that is positive (the current token, already appended, is one of them).  cache:
+    NSADecodeCache or NSAPagedDecodeCache; its compressed rows are not read, so any block / stride will do.  Returns
+    out [B,Hq,Dv]; with return_lse also the float32 [B,Hq] natural-log log-sum-exp of the scaled scores, with which
+    results over disjoint sets of keys can be joined.  A sequence without tokens yields zeros and -inf.
+
+    The tokens of all sequences are cut into equal pieces from the lengths on the device: few long sequences fill the
+    card, a ragged batch does not wait for its longest, and a captured call stays right while the sequences grow.
+    out [B,Hq,Dv] / lse float32 [B,Hq]: result buffers of the caller (allocated here when None)."""
+    _need_cuda(q)
+    if q.dim() != 3 or q.shape[0] != cache.batch or q.shape[2] != cache.dk:
+        raise ValueError("q must be [B,Hq,Dk] = [%d,Hq,%d], got %s" % (cache.batch, cache.dk, tuple(q.shape)))
+    B, hq, dk = q.shape
+    paged = isinstance(cache, NSAPagedDecodeCache)
+    k_c, v_c = (cache.k_pool, cache.v_pool_t) if paged else (cache.k, cache.vt)
+    if q.dtype != k_c.dtype or q.device != k_c.device:
+        raise ValueError("q is %s on %s, the cache %s on %s" % (q.dtype, q.device, k_c.dtype, k_c.device))
+    if hq % cache.hkv:
+        raise ValueError("%d query heads do not share %d kv heads evenly" % (hq, cache.hkv))
+    q = _dense(q)
+    if scale is None:
+        scale = 1.0 / math.sqrt(dk)
+    if out is None:
+        out = torch.empty(B, hq, cache.dv, dtype=q.dtype, device=q.device)
+    elif out.shape != (B, hq, cache.dv) or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        raise ValueError("out must be a contiguous [B,Hq,Dv] tensor of q's dtype and device")
+    if lse is None:
+        lse = torch.empty(B, hq, dtype=torch.float32, device=q.device) if return_lse else None
+    elif lse.shape != (B, hq) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
+        raise ValueError("lse must be a contiguous float32 [B,Hq] tensor on q's device")
+    lib, code = _lib.load(), _dtype_code(q)
+    with _on_device_of(q):
+        need = lib.nsa_dense_decode_workspace_bytes(B, hq, cache.hkv, dk, cache.dv, cache.ctx_cap, sliding_window, code)
+        # a workspace of this call's own: two captured graphs, or two streams, never share one
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+        rc = lib.nsa_dense_decode_step(
+            _ptr(q), _ptr(k_c), _ptr(v_c), _ptr(cache.block_table) if paged else None, cache.max_pages if paged else 0,
+            cache.num_pages if paged else 0, _ptr(cache.ctx_lens), _ptr(out), _ptr(lse), B, hq, cache.hkv, dk, cache.dv,
+            cache.ctx_cap, sliding_window, float(scale), code, _ptr(ws), max(need, 0), _stream())
+    _lib.check(rc, "nsa_dense_decode_step")
+    return (out, lse) if return_lse else out
 
 
 class NSADecodeGraph:

@@ -2,6 +2,7 @@
 enqueue the kernels on the current stream.  No arithmetic happens in Python."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 import os
@@ -34,6 +35,13 @@ def _need_cuda(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:
             raise RuntimeError("NSA kernels run on the GPU only; got a %s tensor" % t.device)
+
+
+def _on_device_of(t: torch.Tensor):
+    """Makes t's GPU the current one for a launch, so that the current stream is one of that GPU."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 def _dense(t: torch.Tensor) -> torch.Tensor:

@@ -1,0 +1,290 @@
+"""GPU tests of dense decode attention (one new token attends every cached token of a contiguous or paged cache) against a
+plain float64 softmax over the same cached tokens.
+
+Bound of the error, from the roundings the kernel makes (u = eps / 2 of the tensors' type, f = 2^-24 of fp32):
+  scores    a sum of dk products in fp32, times the scale: |ds| <= (dk + 8) f |scale| sum |q k|
+  p         off by 2 ds (numerator and denominator) and by 2^-21 (the exponential), then rounded to the tensors' type: u
+  sums      a wavefront adds a quarter of the visible keys one after another at worst, then joins: (n / 4 + 64) f
+  out       rounded once: u |out|
+With A = sum p |v| / l, |out - exact| <= u (|out| + A) + A (4 ds + 2^-20 + 2 (n / 4 + 64) f); the same terms without v for
+the log-sum-exp."""
+import math
+import random
+
+import pytest
+import torch
+
+from tests.util import randn
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F = 2.0 ** -24
+
+
+def make_cache(paged, lens, cap, hkv, dk, dv, dtype, seed, garbage=None):
+    """A cache whose sequences hold lens[b] random tokens; everything else in it is `garbage` (or random)."""
+    from nsa_amd.decode import NSADecodeCache, NSAPagedDecodeCache
+    B = len(lens)
+    ks = [randn(n, hkv, dk, seed=seed + 2 * b, scale=0.7, dtype=dtype) for b, n in enumerate(lens)]
+    vs = [randn(n, hkv, dv, seed=seed + 2 * b + 1, dtype=dtype) for b, n in enumerate(lens)]
+    if paged:
+        need = [(n + 63) // 64 for n in lens]
+        c = NSAPagedDecodeCache(B, sum(need) + 2, cap, hkv, dk, dv, dtype=dtype, device=DEV)
+        ids = list(range(1, sum(need) + 3))
+        random.Random(seed).shuffle(ids)
+        table = torch.zeros(B, c.max_pages, dtype=torch.int32)
+        k_pool = torch.full(c.k_pool.shape, garbage if garbage is not None else 0.0).to(dtype)
+        v_pool = torch.full(c.v_pool_t.shape, garbage if garbage is not None else 0.0).to(dtype)
+        for b, n in enumerate(lens):
+            for p in range(need[b]):
+                pg = ids.pop()
+                table[b, p] = pg
+                m = min(64, n - 64 * p)
+                k_pool[pg, :m] = ks[b][64 * p:64 * p + m]
+                v_pool[pg, :, :, :m] = vs[b][64 * p:64 * p + m].permute(1, 2, 0)
+        c.k_pool.copy_(k_pool)
+        c.v_pool_t.copy_(v_pool)
+        c.block_table.copy_(table)
+    else:
+        c = NSADecodeCache(B, cap, hkv, dk, dv, dtype=dtype, device=DEV)
+        if garbage is not None:
+            c.k.fill_(garbage)
+            c.vt.fill_(garbage)
+        for b, n in enumerate(lens):
+            c.k[b, :n] = ks[b].to(DEV)
+            c.vt[b, :, :, :n] = vs[b].permute(1, 2, 0).to(DEV)
+    c.ctx_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+    return c, ks, vs
+
+
+def plain(q, k, v, scale, window):
+    """q [Hq,Dk], k [n,Hkv,Dk], v [n,Hkv,Dv] -> float64 out [Hq,Dv], lse [Hq] and the error bounds of both."""
+    hq, hkv, n = q.shape[0], k.shape[1], k.shape[0]
+    u = torch.finfo(q.dtype).eps / 2
+    lo = max(0, n - window) if window else 0
+    q, k, v = q.double(), k.double()[lo:], v.double()[lo:]
+    if n == 0:
+        z = torch.zeros(hq, v.shape[2], dtype=torch.float64, device=q.device)
+        return z, torch.full((hq,), -math.inf, dtype=torch.float64, device=q.device), z, z[:, 0]
+    qg = q.view(hkv, hq // hkv, -1)
+    kt = k.permute(1, 2, 0).contiguous()
+    vh = v.transpose(0, 1).contiguous()
+    s = scale * torch.matmul(qg, kt)
+    p = torch.softmax(s, -1)
+    out = torch.matmul(p, vh).reshape(hq, -1)
+    A = torch.matmul(p, vh.abs()).reshape(hq, -1)
+    lse = torch.logsumexp(s, -1).reshape(hq)
+    ds = ((q.shape[1] + 8) * F * abs(scale) * torch.matmul(qg.abs(), kt.abs()).amax(-1)).reshape(hq)
+    chain = 2 * ((n - lo) / 4 + 64) * F
+    tol = u * (out.abs() + A) + A * (4 * ds[:, None] + 2.0 ** -20 + chain)
+    tol_lse = 2 * ds + 2.0 ** -20 + chain + 4 * F * lse.abs()
+    return out, lse, tol, tol_lse
+
+
+def check(q, c, ks, vs, window=0, scale=None, **kw):
+    from nsa_amd.decode import dense_decode_step
+    out, lse = dense_decode_step(q, c, scale=scale, sliding_window=window, return_lse=True, **kw)
+    assert out.dtype == q.dtype and out.shape == (q.shape[0], q.shape[1], c.dv) and lse.shape == q.shape[:2]
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    got, got_lse = out.double().cpu(), lse.double().cpu()
+    for b in range(len(ks)):
+        ref, ref_lse, tol, tol_lse = plain(q[b].cpu(), ks[b], vs[b], scale, window)
+        assert torch.isfinite(got[b]).all(), b
+        assert ((got[b] - ref).abs() <= tol).all(), (b, len(ks[b]), float(((got[b] - ref).abs() / tol).max()))
+        if len(ks[b]) == 0:
+            assert (got[b] == 0).all() and (got_lse[b] == -math.inf).all()
+        else:
+            assert ((got_lse[b] - ref_lse).abs() <= tol_lse).all(), (b, len(ks[b]))
+    return out, lse
+
+
+LENS = [700, 0, 1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 191, 257, 1000, 2049]
+
+
+@pytest.mark.parametrize("paged", [True, False])
+@pytest.mark.parametrize("dtype,hq,hkv,dk,dv", [
+    (torch.bfloat16, 64, 4, 128, 128),
+    (torch.float16, 24, 2, 192, 128),
+    (torch.bfloat16, 8, 8, 64, 64),
+    (torch.float32, 4, 1, 64, 64),
+    (torch.float32, 16, 2, 128, 128),
+    (torch.float32, 6, 1, 192, 128),
+    (torch.float16, 4, 2, 32, 32),
+])
+@pytest.mark.parametrize("window", [0, 1, 100])
+def test_every_length(paged, dtype, hq, hkv, dk, dv, window):
+    c, ks, vs = make_cache(paged, LENS, 2112, hkv, dk, dv, dtype, seed=10)
+    q = randn(len(LENS), hq, dk, seed=9, dtype=dtype).to(DEV)
+    check(q, c, ks, vs, window)
+
+
+@pytest.mark.parametrize("dtype,dk,dv", [(torch.bfloat16, 128, 128), (torch.float32, 64, 64), (torch.bfloat16, 192, 128),
+                                         (torch.float32, 192, 128)])
+@pytest.mark.parametrize("group", [1, 2, 3, 7, 15, 16, 17, 24, 32, 33, 48, 64, 65, 80, 130])
+def test_every_group_size(dtype, dk, dv, group):
+    lens = [300, 77, 1]
+    c, ks, vs = make_cache(True, lens, 320, 2, dk, dv, dtype, seed=30)
+    q = randn(len(lens), 2 * group, dk, seed=29, dtype=dtype).to(DEV)
+    check(q, c, ks, vs)
+
+
+@pytest.mark.parametrize("paged", [True, False])
+@pytest.mark.parametrize("garbage", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_what_lies_behind_a_sequence_does_not_matter(paged, garbage, dtype):
+    lens = [1, 5, 32, 40, 64, 70, 100, 0, 333]
+    c, ks, vs = make_cache(paged, lens, 384, 2, 64, 64, dtype, seed=50, garbage=garbage)
+    q = randn(len(lens), 8, 64, seed=49, dtype=dtype).to(DEV)
+    check(q, c, ks, vs)
+    # and what lies before the window
+    for b, n in enumerate(lens):
+        for j in range(max(0, n - 37)):
+            if paged:
+                c.k_pool[c.block_table[b, j // 64].long(), j % 64] = garbage
+                c.v_pool_t[c.block_table[b, j // 64].long(), :, :, j % 64] = garbage
+            else:
+                c.k[b, j] = garbage
+                c.vt[b, :, :, j] = garbage
+    check(q, c, ks, vs, window=37)
+
+
+def test_lowest_values_as_scores_and_large_scores():
+    """Scores at the ends of the range: one key far above the others, and all of them equally low."""
+    dtype = torch.float32
+    lens = [200, 200]
+    c, ks, vs = make_cache(True, lens, 256, 1, 64, 64, dtype, seed=60)
+    q = randn(2, 4, 64, seed=61, dtype=dtype).to(DEV)
+    for scale in (-0.125, 0.0, 30.0):
+        check(q, c, ks, vs, scale=scale)
+
+
+@pytest.mark.parametrize("paged", [True, False])
+def test_many_sequences(paged):
+    """more sequences than a wavefront has lanes, most of them empty or short, a few long"""
+    g = random.Random(3)
+    lens = [g.choice([0, 0, 1, 5, 64, 130]) for _ in range(203)]
+    lens[70], lens[202] = 3000, 2500
+    c, ks, vs = make_cache(paged, lens, 3008, 2, 64, 64, torch.bfloat16, seed=70)
+    q = randn(len(lens), 16, 64, seed=69, dtype=torch.bfloat16).to(DEV)
+    check(q, c, ks, vs)
+
+
+def test_units_of_more_pages_than_a_wavefront_has_lanes():
+    """64 kv heads leave 16 units for 1500 pages, so a unit's page ids are read in several runs"""
+    from nsa_amd.decode import NSAPagedDecodeCache, dense_decode_step
+    H, D, n, dtype = 64, 32, 95_990, torch.bfloat16
+    P = (n + 63) // 64
+    c = NSAPagedDecodeCache(2, P + 1, n, H, D, D, dtype=dtype, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    c.k_pool.copy_(torch.randn(c.k_pool.shape, generator=gen, device=DEV, dtype=dtype))
+    c.v_pool_t.copy_(torch.randn(c.v_pool_t.shape, generator=gen, device=DEV, dtype=dtype))
+    order = torch.randperm(P, generator=torch.Generator().manual_seed(5)) + 1
+    c.block_table[0, :P] = order.int().to(DEV)
+    c.block_table[1, 0] = P + 1
+    c.ctx_lens.copy_(torch.tensor([n, 50], dtype=torch.int32))
+    q = torch.randn(2, H, D, generator=gen, device=DEV, dtype=dtype)
+    out, lse = dense_decode_step(q, c, return_lse=True)
+    for b, m in ((0, n), (1, 50)):
+        ids = c.block_table[b, :(m + 63) // 64].long()
+        for h in range(0, H, 9):
+            k = c.k_pool[ids, :, h].reshape(-1, 1, D)[:m]
+            v = c.v_pool_t[ids, h].transpose(1, 2).reshape(-1, 1, D)[:m]
+            ref, ref_lse, tol, tol_lse = plain(q[b, h:h + 1], k, v, D ** -0.5, 0)
+            assert ((out[b, h:h + 1].double() - ref).abs() <= tol).all()
+            assert ((lse[b, h:h + 1].double() - ref_lse).abs() <= tol_lse).all()
+
+
+def test_offsets_beyond_32_bits():
+    """pages behind element 2^31 of both pools"""
+    from nsa_amd.decode import NSAPagedDecodeCache, dense_decode_step
+    H, D, dtype = 4, 128, torch.bfloat16
+    pages = 2 ** 31 // (64 * H * D) + 40
+    c = NSAPagedDecodeCache(1, pages, 2048, H, D, D, dtype=dtype, device=DEV)
+    n = 32 * 64 - 11
+    k = randn(2048, H, D, seed=80, dtype=dtype)
+    v = randn(2048, H, D, seed=81, dtype=dtype)
+    c.k_pool[pages - 31:] = k.view(32, 64, H, D).to(DEV)
+    c.v_pool_t[pages - 31:] = v.view(32, 64, H, D).permute(0, 2, 3, 1).to(DEV)
+    c.block_table[0] = torch.arange(pages - 31, pages + 1, dtype=torch.int32, device=DEV)
+    c.ctx_lens.fill_(n)
+    q = randn(1, 64, D, seed=82, dtype=dtype).to(DEV)
+    check(q, c, [k[:n]], [v[:n]])
+
+
+def test_lengths_and_page_ids_outside_the_cache_stay_inside_it():
+    """a length beyond the capacity counts as the capacity, a negative one as 0; an id outside the pool reads page 0"""
+    from nsa_amd.decode import dense_decode_step
+    lens = [128, 128, 128]
+    c, ks, vs = make_cache(True, lens, 128, 2, 64, 64, torch.bfloat16, seed=90)
+    q = randn(3, 8, 64, seed=91, dtype=torch.bfloat16).to(DEV)
+    want = dense_decode_step(q, c)
+    c.ctx_lens.copy_(torch.tensor([129, 10 ** 6, -5], dtype=torch.int32))
+    out, lse = dense_decode_step(q, c, return_lse=True)
+    assert torch.equal(out[:2], want[:2]) and (out[2] == 0).all() and (lse[2] == -math.inf).all()
+    c.ctx_lens.fill_(128)
+    c.block_table[0, 1] = c.num_pages
+    c.block_table[1, 1] = -1
+    got = dense_decode_step(q, c)
+    c.block_table[:2, 1] = 0
+    assert torch.equal(got, dense_decode_step(q, c))
+
+
+@pytest.mark.parametrize("window", [0, 200])
+def test_equals_the_last_row_of_the_prefill_kernels(window):
+    """the same token through sliding_window_attn, whose window covers the whole prompt or part of it"""
+    import nsa_amd
+    from nsa_amd.decode import NSADecodeCache, dense_decode_step
+    T, hq, hkv, D, dtype = 777, 16, 2, 128, torch.bfloat16
+    q, k, v = (randn(1, T, h, D, seed=100 + h, dtype=dtype).to(DEV) for h in (hq, hkv, hkv))
+    rows = nsa_amd.sliding_window_attn(q, k, v, window or T)
+    c = NSADecodeCache(1, T, hkv, D, D, dtype=dtype, device=DEV)
+    c.fill(k, v)
+    out = dense_decode_step(q[:, -1], c, sliding_window=window)
+    u = torch.finfo(dtype).eps / 2      # both sides: probabilities and output rounded (|v| < 5, the weights sum to 1)
+    assert float((out.double() - rows[:, -1].double()).abs().max()) <= 2 * u * (5 + float(rows.abs().max()))
+
+
+def test_buffers_strides_and_streams():
+    from nsa_amd.decode import dense_decode_step
+    lens = [500, 3]
+    c, ks, vs = make_cache(True, lens, 512, 2, 64, 64, torch.bfloat16, seed=110)
+    wide = randn(2, 8, 3, 64, seed=111, dtype=torch.bfloat16).to(DEV)
+    q = wide[:, :, 1]                                       # heads 3 * 64 apart
+    want, want_lse = check(q, c, ks, vs)
+    out = torch.full((2, 8, 64), 7.0, dtype=torch.bfloat16, device=DEV)
+    lse = torch.full((2, 8), 7.0, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        a = dense_decode_step(q, c, out=out, lse=lse)
+        b = dense_decode_step(q, c)
+    torch.cuda.current_stream().wait_stream(side)
+    assert a is out and torch.equal(out, want) and torch.equal(lse, want_lse) and torch.equal(b, want)
+
+
+def test_captured_calls_follow_the_growing_cache():
+    """two graphs captured over the same cache, replayed in turn while the sequences grow, equal the eager calls"""
+    from nsa_amd.decode import NSAPagedDecodeCache, dense_decode_step
+    B, hq, hkv, D, dtype, T0, steps = 3, 16, 2, 128, torch.bfloat16, 600, 70
+    c = NSAPagedDecodeCache(B, 40, 768, hkv, D, D, dtype=dtype, device=DEV)
+    k, v = (randn(B, T0 + steps, hkv, D, seed=120 + i, dtype=dtype).to(DEV) for i in range(2))
+    q = randn(steps, B, hq, D, seed=122, dtype=dtype).to(DEV)
+    c.fill(k[:, :T0], v[:, :T0])
+    fixed = torch.zeros(B, hq, D, dtype=dtype, device=DEV)
+    graphs, outs = [], []
+    for window in (0, 100):
+        dense_decode_step(fixed, c, sliding_window=window)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(dense_decode_step(fixed, c, sliding_window=window))
+        graphs.append(g)
+    for s in range(steps):
+        c.append(k[:, T0 + s], v[:, T0 + s])
+        fixed.copy_(q[s])
+        for g, out, window in zip(graphs, outs, (0, 100)):
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, dense_decode_step(q[s], c, sliding_window=window)), (s, window)
+    for b in range(B):
+        ref, _, tol, _ = plain(q[-1, b].cpu(), k[b].cpu(), v[b].cpu(), D ** -0.5, 0)
+        assert ((outs[0][b].double().cpu() - ref).abs() <= tol).all()
