@@ -32,27 +32,77 @@ __device__ __forceinline__ DenseSpan dense_span(int len, int cap, int window) {
   s.pages = ((s.n + 63) >> 6) - s.first;
   return s;
 }
+// Sum over the wavefront, in every lane: rotations inside the 16-lane rows, then the two row exchanges.
 __device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x128, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x124, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x122, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x121, 0xF, 0xF, true);
+  auto r = __builtin_amdgcn_permlane16_swap((unsigned)x, (unsigned)x, false, false);
+  x = (int)(r[0] + r[1]);
+  r = __builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)x, false, false);
+  return (int)(r[0] + r[1]);
+}
+// Inclusive prefix sum over the wavefront: shifts inside the rows, then the last lane of row 0 and 2 added to the row
+// behind it, and that of row 1 to rows 2 and 3.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
   return x;
 }
-// Pages per unit: the pages of all sequences over the units aimed at.  sum_b max(1, ceil(pages_b / C)) is then at most
-// units + batch, which is what the grid and the workspace hold.
-__device__ __forceinline__ int dense_unit_pages(const DenseDecodeArgs& a) {
-  int total = 0;
-  for (int b = __lane_id(); b < a.batch; b += 64) total += dense_span(a.ctx_lens[b], a.ctx_cap, a.window).pages;
-  total = wave_sum(total);
-  return max(kDenseMinPages, (int)(((unsigned)total + a.units - 1) / (unsigned)a.units));
-}
 __device__ __forceinline__ int dense_units_of(int pages, int C) { return max(1, (int)((unsigned)(pages + C - 1) / (unsigned)C)); }
+// Pages per unit: the pages of all sequences over the units aimed at, and more where a ragged batch's last, shorter
+// units would make a second round of workgroups (each step takes C up by the excess).  sum_b max(1, ceil(pages_b / C)) is
+// at most units + batch for the first C already, which is what the grid and the workspace hold.
+__device__ __forceinline__ int dense_unit_pages(const DenseDecodeArgs& a) {
+  const int lane = __lane_id();
+  if (a.batch == 1) {
+    const unsigned pages = dense_span(a.ctx_lens[0], a.ctx_cap, a.window).pages;
+    return max(kDenseMinPages, (int)((pages + a.units - 1) / (unsigned)a.units));
+  }
+  int total = 0, mine = 0;
+  for (int b = lane; b < a.batch; b += 64) {
+    mine = dense_span(a.ctx_lens[b], a.ctx_cap, a.window).pages;
+    total += mine;
+  }
+  total = wave_sum(total);
+  const unsigned aim = (unsigned)a.units;
+  int C = max(kDenseMinPages, (int)(((unsigned)total + aim - 1) / aim));
+  if (a.batch > 64 || a.batch >= a.units) return C;
+#pragma unroll 1
+  for (int step = 0; step < 3; ++step) {
+    const unsigned got = wave_sum(lane < a.batch ? dense_units_of(mine, C) : 0);
+    if (got <= aim) break;
+    C = max(C + 1, (int)(((uint64_t)C * got + aim - 1) / aim));
+  }
+  return C;
+}
 
-// Visible keys of the chunk [cb, cb + 32) are lo..n-1.  Whatever a page holds outside them (rows of a sequence that
-// had the page before, infinities, NaN) must not reach the sums: their scores are replaced, and their values too,
-// since 0 * inf is NaN.
+// Fragments of one 32-key chunk and the two products on them.  Visible keys of the chunk [cb, cb + 32) are lo..n-1.
+// Whatever a page holds outside them (rows of a sequence that had the page before, infinities, NaN) must not reach the
+// sums: their scores are replaced, and their values too, since 0 * inf is NaN.
+template <typename T, int DK, int NT>
+__device__ __forceinline__ void dense_scores(const vec8_t<T> (&k0)[DK / 32], const vec8_t<T> (&k1)[DK / 32],
+                                             const vec8_t<T> (&q)[NT][DK / 32], float (&s)[NT][8]) {
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    f32x4_t s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kk = 0; kk < DK / 32; ++kk) {
+      s0 = mma16(k0[kk], q[j][kk], s0);
+      s1 = mma16(k1[kk], q[j][kk], s1);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { s[j][i] = s0[i]; s[j][4 + i] = s1[i]; }
+  }
+}
 template <typename T, int DK, int DV, int NT>
-__device__ __forceinline__ void dense_attend(DecState<T, DK, DV> (&st)[NT], ChunkFrags<T, DK, DV>& f,
-                                             const vec8_t<T> (&q)[NT][DK / 32], int cb, int lo, int n, float c, int g) {
+__device__ __forceinline__ void dense_values(DecState<T, DK, DV> (&st)[NT], vec8_t<T> (&v)[DV / 16],
+                                             const float (&s)[NT][8], int cb, int lo, int n, float c, int g) {
   const bool whole = cb >= lo && cb + 32 <= n;
   if (!whole) {
 #pragma unroll
@@ -60,32 +110,19 @@ __device__ __forceinline__ void dense_attend(DecState<T, DK, DV> (&st)[NT], Chun
       const int key = cb + 8 * g + i;
       if (key < lo || key >= n) {
 #pragma unroll
-        for (int t = 0; t < DV / 16; ++t) f.v[t][i] = (T)0.0f;
+        for (int t = 0; t < DV / 16; ++t) v[t][i] = (T)0.0f;
       }
     }
   }
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
-    f32x4_t s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int kk = 0; kk < DK / 32; ++kk) {
-      s0 = mma16(f.k0[kk], q[j][kk], s0);
-      s1 = mma16(f.k1[kk], q[j][kk], s1);
-    }
-    float s[8], p[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { s[i] = s0[i]; s[4 + i] = s1[i]; }
+    float p[8];
     float mx = kNegInf;
-    if (whole) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, s[i] * c);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int key = cb + 8 * g + i;
-        const bool seen = key >= lo && key < n;
-        mx = fmaxf(mx, seen ? s[i] * c : kNegInf);
-      }
+    for (int i = 0; i < 8; ++i) {
+      const int key = cb + 8 * g + i;
+      const float x = s[j][i] * c;
+      mx = fmaxf(mx, whole || (key >= lo && key < n) ? x : kNegInf);
     }
     const float m_new = fmaxf(st[j].m, colgroup_max(mx));
     const float mref = m_new == kNegInf ? 0.f : m_new;
@@ -94,33 +131,30 @@ __device__ __forceinline__ void dense_attend(DecState<T, DK, DV> (&st)[NT], Chun
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int key = cb + 8 * g + i;
-      p[i] = fast_exp2(fmaf(s[i], c, -mref));
-      if (!whole && (key < lo || key >= n)) p[i] = 0.f;
+      const float x = fast_exp2(fmaf(s[j][i], c, -mref));
+      p[i] = whole || (key >= lo && key < n) ? x : 0.f;
       sum += p[i];
     }
     st[j].l = st[j].l * alpha + sum;
     st[j].m = m_new;
-    // probabilities are rounded to the tensors' type for the second product (at most 2^-9 of each at bf16, the
+    // probabilities are rounded to the tensors' type for the second product (at most half a step of each, the
     // denominator keeps fp32); the sums stay in fp32
     const vec8_t<T> pb = pack8<T>(p);
 #pragma unroll
     for (int t = 0; t < DV / 16; ++t) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) st[j].o[t][i] *= alpha;
-      st[j].o[t] = mma16(f.v[t], pb, st[j].o[t]);
+      st[j].o[t] = mma16(v[t], pb, st[j].o[t]);
     }
   }
 }
 
-// Registers (32-bit, per lane) of one chunk's fragments, and of the queries and sums of NT head tiles.
-template <typename T, int DK, int DV> constexpr int kDenseFragRegs = (2 * (DK / 32) + DV / 16) * 2 * (int)sizeof(T);
-template <typename T, int DK, int DV, int NT> constexpr int kDenseTileRegs = NT * ((DK / 32) * 2 * (int)sizeof(T) + DV / 4);
-// A second chunk in flight while one is worked on, where the register file (512 per lane) holds both.
-template <typename T, int DK, int DV, int NT> constexpr bool kDenseAhead =
-    2 * kDenseFragRegs<T, DK, DV> + kDenseTileRegs<T, DK, DV, NT> <= 384;
-// Two wavefronts per SIMD where 256 registers hold that.
+// Registers (32-bit, per lane) of one chunk's fragments, of the queries and sums of NT head tiles, and what else there is.
+template <typename T, int DK, int DV, int NT> constexpr int kDenseRegs =
+    (2 * (DK / 32) + DV / 16) * 2 * (int)sizeof(T) + NT * ((DK / 32) * 2 * (int)sizeof(T) + DV / 4) + 48;
+// Wavefronts per SIMD that the register file (512) then holds.
 template <typename T, int DK, int DV, int NT> constexpr int kDenseOccupancy =
-    2 * kDenseFragRegs<T, DK, DV> + kDenseTileRegs<T, DK, DV, NT> <= 192 ? 2 : 1;
+    kDenseRegs<T, DK, DV, NT> <= 128 ? 4 : kDenseRegs<T, DK, DV, NT> <= 168 ? 3 : kDenseRegs<T, DK, DV, NT> <= 256 ? 2 : 1;
 
 // NT: 16-head tiles of the GQA group that share the loaded keys and values.  grid: unit * (hkv * head blocks) + those
 template <typename T, int DK, int DV, int NT>
@@ -142,12 +176,7 @@ dense_decode_kernel(const DenseDecodeArgs a) {
   for (int b0 = 0; b0 < a.batch && b < 0; b0 += 64) {
     const int mine = b0 + lane;
     const int nu = mine < a.batch ? dense_units_of(dense_span(a.ctx_lens[mine], a.ctx_cap, a.window).pages, C) : 0;
-    int incl = nu;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int up = __shfl_up(incl, d);
-      if (lane >= d) incl += up;
-    }
+    const int incl = wave_scan(nu);
     const int run = __builtin_amdgcn_readlane(incl, 63);
     if (unit < before + run) {
       const unsigned long long hit = __ballot(before + incl > unit);
@@ -185,48 +214,49 @@ dense_decode_kernel(const DenseDecodeArgs a) {
   // chunk i of this wavefront covers keys 64 p0 + 32 (w + 4 i) ..; 64 page ids at a time sit in the lanes
   int ids_at = p0, ids = 0;
   if (paged && p0 + lane < p1) ids = table[p0 + lane];
-  ChunkFrags<T, DK, DV> f[kDenseAhead<T, DK, DV, NT> ? 2 : 1];
-  auto issue = [&](ChunkFrags<T, DK, DV>& fr, int cb) {
+  auto page_of = [&](int cb) -> int {
     const int p = cb >> 6;
-    const T *kp, *vp;
-    if (paged) {
-      if (p - ids_at >= 64) {
-        ids_at = p;
-        ids = p + lane < p1 ? table[p + lane] : 0;
-      }
-      // an id outside the pool would fault: read page 0 instead (the caller's table is wrong)
-      int id = __builtin_amdgcn_readlane(ids, p - ids_at);
-      id = (unsigned)id < (unsigned)a.num_pages ? id : 0;
-      kp = kbase + ((long)id * 64 + (cb & 63)) * krow;
-      vp = vbase + ((long)id * a.hkv + h) * DV * 64 + (cb & 63);
-    } else {
-      kp = kbase + ((long)b * a.ctx_cap + cb) * krow;
-      vp = vbase + ((long)b * a.hkv + h) * DV * vrow + cb;
+    if (p - ids_at >= 64) {
+      ids_at = p;
+      ids = p + lane < p1 ? table[p + lane] : 0;
     }
+    // an id outside the pool would fault: read page 0 instead (the caller's table is wrong)
+    const int id = __builtin_amdgcn_readlane(ids, p - ids_at);
+    return (unsigned)id < (unsigned)a.num_pages ? id : 0;
+  };
+  vec8_t<T> k0[DK / 32], k1[DK / 32], v[DV / 16];
+  auto load_keys = [&](int cb, int id) {
+    const T* kp = kbase + (paged ? (long)id * 64 + (cb & 63) : (long)b * a.ctx_cap + cb) * krow;
     const T* k0p = kp + chunk_key_of_row(0, n16) * krow;
     const T* k1p = kp + chunk_key_of_row(1, n16) * krow;
 #pragma unroll
-    for (int kk = 0; kk < DK / 32; ++kk) { fr.k0[kk] = load8(k0p + 32 * kk); fr.k1[kk] = load8(k1p + 32 * kk); }
-    vp += (long)n16 * vrow + 8 * g;
-#pragma unroll
-    for (int t = 0; t < DV / 16; ++t) fr.v[t] = load8(vp + 16 * t * vrow);
+    for (int kk = 0; kk < DK / 32; ++kk) { k0[kk] = load8(k0p + 32 * kk); k1[kk] = load8(k1p + 32 * kk); }
   };
+  auto load_values = [&](int cb, int id) {
+    const T* vp = vbase + ((long)(paged ? id : b) * a.hkv + h) * DV * vrow + (paged ? (cb & 63) : cb) + (long)n16 * vrow + 8 * g;
+#pragma unroll
+    for (int t = 0; t < DV / 16; ++t) v[t] = load8(vp + 16 * t * vrow);
+  };
+  // the next chunk's keys are requested as soon as the scores have used this one's, its values after the second
+  // product: one set of registers, and loads of this wavefront are always in flight
   const int end = min(p1 * 64, sp.n);
   int cb = p0 * 64 + 32 * w;
-  if constexpr (kDenseAhead<T, DK, DV, NT>) {
-    if (cb < end) issue(f[0], cb);
-    while (cb < end) {
-      const int c1 = cb + 32 * kDenseWaves, c2 = c1 + 32 * kDenseWaves;
-      if (c1 < end) issue(f[1], c1);
-      dense_attend<T, DK, DV, NT>(st, f[0], q, cb, sp.lo, sp.n, c, g);
-      if (c2 < end) issue(f[0], c2);
-      if (c1 < end) dense_attend<T, DK, DV, NT>(st, f[1], q, c1, sp.lo, sp.n, c, g);
-      cb = c2;
-    }
-  } else {
-    for (; cb < end; cb += 32 * kDenseWaves) {
-      issue(f[0], cb);
-      dense_attend<T, DK, DV, NT>(st, f[0], q, cb, sp.lo, sp.n, c, g);
+  if (cb < end) {
+    int id = paged ? page_of(cb) : 0;
+    load_keys(cb, id);
+    load_values(cb, id);
+    while (true) {
+      float s[NT][8];
+      dense_scores<T, DK, NT>(k0, k1, q, s);
+      const int next = cb + 32 * kDenseWaves;
+      if (next < end) {
+        id = paged ? page_of(next) : 0;
+        load_keys(next, id);
+      }
+      dense_values<T, DK, DV, NT>(st, v, s, cb, sp.lo, sp.n, c, g);
+      if (next >= end) break;
+      load_values(next, id);
+      cb = next;
     }
   }
 
@@ -289,7 +319,7 @@ __global__ void __launch_bounds__(256)
 dense_decode_join_kernel(const DenseDecodeArgs a, int rows_per_slot, int blocks) {
   constexpr int kLanes = DV / 4, kGroups = 256 / kLanes;
   __shared__ float acc[kGroups][DV];
-  __shared__ float red[kGroups];
+  __shared__ float red[kGroups][2];
   const int b = blockIdx.x / a.hq, head = blockIdx.x % a.hq;
   const int lane = threadIdx.x & 63;
   const int C = dense_unit_pages(a);
@@ -302,31 +332,57 @@ dense_decode_join_kernel(const DenseDecodeArgs a, int rows_per_slot, int blocks)
   const int per = a.hkv * blocks, hb = h * blocks + r / rows_per_slot;
   const long step = (long)per * rows_per_slot;
   const long first = ((long)u0 * per + hb) * rows_per_slot + r % rows_per_slot;
-  float M = kNegInf;
-  for (int u = lane; u < count; u += 64) M = fmaxf(M, a.part_ml[(first + u * step) * 2]);
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
+  // every kLanes threads run over their own units, eight at a time so that the loads of a round travel together
   const int x = threadIdx.x % kLanes, y = threadIdx.x / kLanes;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  float L = 0.f;
-  for (int u = y; u < count; u += kGroups) {
-    const long at = first + u * step;
-    const float wgt = M == kNegInf ? 0.f : fast_exp2(a.part_ml[at * 2] - M);
-    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(a.part + at * DV + 4 * x);
+  float m = kNegInf, l = 0.f;
+  for (int u = y; u < count; u += 8 * kGroups) {
+    float um[8], ul[8];
+    f32x4_t uo[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = fmaf(v[i], wgt, o[i]);
-    L = fmaf(a.part_ml[at * 2 + 1], wgt, L);
+    for (int k = 0; k < 8; ++k) {
+      const long at = first + min(u + k * kGroups, count - 1) * step;
+      um[k] = a.part_ml[at * 2];
+      ul[k] = a.part_ml[at * 2 + 1];
+      uo[k] = *reinterpret_cast<const f32x4_t*>(a.part + at * DV + 4 * x);
+    }
+    float mx = m;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (u + k * kGroups >= count) um[k] = kNegInf;       // the last unit once more
+      mx = fmaxf(mx, um[k]);
+    }
+    const float ref = mx == kNegInf ? 0.f : mx;
+    const float alpha = fast_exp2(m - ref);
+    m = mx;
+    l *= alpha;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] *= alpha;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float wgt = fast_exp2(um[k] - ref);
+      l = fmaf(ul[k], wgt, l);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = fmaf(uo[k][i], wgt, o[i]);
+    }
   }
   *reinterpret_cast<f32x4_t*>(&acc[y][4 * x]) = o;
-  if (x == 0) red[y] = L;
+  if (x == 0) { red[y][0] = m; red[y][1] = l; }
   __syncthreads();
   if (threadIdx.x >= DV) return;
-  float sum = 0.f, l = 0.f;
+  float M = kNegInf, sum = 0.f, L = 0.f;
 #pragma unroll
-  for (int k = 0; k < kGroups; ++k) { sum += acc[k][threadIdx.x]; l += red[k]; }
+  for (int k = 0; k < kGroups; ++k) M = fmaxf(M, red[k][0]);
+  const float ref = M == kNegInf ? 0.f : M;
+#pragma unroll
+  for (int k = 0; k < kGroups; ++k) {
+    const float wgt = fast_exp2(red[k][0] - ref);
+    sum = fmaf(acc[k][threadIdx.x], wgt, sum);
+    L = fmaf(red[k][1], wgt, L);
+  }
   const long row = (long)b * a.hq + head;
-  reinterpret_cast<T*>(a.out)[row * DV + threadIdx.x] = (T)(l > 0.f ? sum / l : 0.f);
-  if (a.lse != nullptr && threadIdx.x == 0) a.lse[row] = l > 0.f ? (M + __log2f(l)) * (1.0f / kLog2e) : kNegInf;
+  reinterpret_cast<T*>(a.out)[row * DV + threadIdx.x] = (T)(L > 0.f ? sum / L : 0.f);
+  if (a.lse != nullptr && threadIdx.x == 0) a.lse[row] = L > 0.f ? (M + __log2f(L)) * (1.0f / kLog2e) : kNegInf;
 }
 
 // 16-head tiles that share one pass over the keys: the whole group up to 64 heads (32 in fp32, whose fragments take
@@ -345,8 +401,12 @@ DensePlan dense_decode_plan(const DenseDecodeArgs& a) {
   const long per = (long)a.hkv * p.blocks;
   const int cap_pages = (a.ctx_cap + 63) / 64;
   const int span = a.window > 0 ? (int)min((long)cap_pages, ((long)a.window + 62) / 64 + 1) : cap_pages;
-  constexpr long kWorkgroups = 1024;
-  p.units = (int)max(1L, min(kWorkgroups / per, (long)a.batch * span));
+  // One workgroup per CU where its four wavefronts keep 64 KB of loads in flight, more where a chunk is smaller: few long
+  // streams reach more of the memory's rate than many (64 sequences of 32768 tokens, 128 / 128 bf16: 722 us with 256
+  // workgroups, 767 with 512, 791 with 768; 16 of them at 64 / 64: 108, 102, 105 us)
+  const long in_flight = 32L * kDenseWaves * (a.dk + a.dv) * (a.dtype == 1 ? 4 : 2);
+  const long workgroups = 256 * min(4L, max(1L, 65536 / in_flight));
+  p.units = (int)max(1L, min(workgroups / per, (long)a.batch * span));
   p.split = span > kDenseMinPages;         // otherwise every sequence is one unit
   p.slots = ((long)p.units + a.batch) * per;
   p.rows = 16 * p.tiles;

@@ -5,13 +5,14 @@ forward over the cached tokens (mean-pool compressor): block importance over eve
 row, top-n blocks, selected + sliding-window + compressed attention, gated sum."""
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional
 
 import torch
 
 from . import _lib
-from .ops import _dense, _dtype_code, _need_cuda, _on_device_of, _ptr, _stream
+from .ops import _dense, _dtype_code, _need_cuda, _ptr, _raw_stream, _stream
 
 
 def _round_up(x: int, m: int) -> int:
@@ -341,7 +342,11 @@ def nsa_decode_step(q: torch.Tensor, cache, gates: Optional[torch.Tensor] = None
     return (out, idx) if return_indices else out
 
 
-@torch.no_grad()
+@functools.lru_cache(maxsize=256)
+def _dense_workspace_bytes(*sizes):
+    return _lib.load().nsa_dense_decode_workspace_bytes(*sizes)
+
+
 def dense_decode_step(q: torch.Tensor, cache, scale: Optional[float] = None, sliding_window: int = 0,
                       return_lse: bool = False, out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None):
     """Full attention of one new token per sequence: q [B,Hq,Dk] attends every cached token of its sequence, or the last
@@ -354,36 +359,44 @@ def dense_decode_step(q: torch.Tensor, cache, scale: Optional[float] = None, sli
     card, a ragged batch does not wait for its longest, and a captured call stays right while the sequences grow.
     out [B,Hq,Dv] / lse float32 [B,Hq]: result buffers of the caller (allocated here when None)."""
     _need_cuda(q)
-    if q.dim() != 3 or q.shape[0] != cache.batch or q.shape[2] != cache.dk:
-        raise ValueError("q must be [B,Hq,Dk] = [%d,Hq,%d], got %s" % (cache.batch, cache.dk, tuple(q.shape)))
-    B, hq, dk = q.shape
-    paged = isinstance(cache, NSAPagedDecodeCache)
+    B, hkv, dv, paged = cache.batch, cache.hkv, cache.dv, isinstance(cache, NSAPagedDecodeCache)
+    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != cache.dk:
+        raise ValueError("q must be [B,Hq,Dk] = [%d,Hq,%d], got %s" % (B, cache.dk, tuple(q.shape)))
+    hq, dk, device = q.shape[1], cache.dk, q.device
     k_c, v_c = (cache.k_pool, cache.v_pool_t) if paged else (cache.k, cache.vt)
-    if q.dtype != k_c.dtype or q.device != k_c.device:
-        raise ValueError("q is %s on %s, the cache %s on %s" % (q.dtype, q.device, k_c.dtype, k_c.device))
-    if hq % cache.hkv:
-        raise ValueError("%d query heads do not share %d kv heads evenly" % (hq, cache.hkv))
+    if q.dtype != k_c.dtype or device != k_c.device:
+        raise ValueError("q is %s on %s, the cache %s on %s" % (q.dtype, device, k_c.dtype, k_c.device))
+    if hq == 0 or hq % hkv:
+        raise ValueError("%d query heads do not share %d kv heads evenly" % (hq, hkv))
+    if sliding_window < 0:
+        raise ValueError("sliding_window must not be negative")
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return dense_decode_step(q, cache, scale, sliding_window, return_lse, out, lse)
     q = _dense(q)
     if scale is None:
         scale = 1.0 / math.sqrt(dk)
     if out is None:
-        out = torch.empty(B, hq, cache.dv, dtype=q.dtype, device=q.device)
-    elif out.shape != (B, hq, cache.dv) or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
-        raise ValueError("out must be a contiguous [B,Hq,Dv] tensor of q's dtype and device")
+        out = torch.empty((B, hq, dv), dtype=q.dtype, device=device)
+    elif out.shape != (B, hq, dv) or out.dtype != q.dtype or out.device != device or not out.is_contiguous() \
+            or out.data_ptr() % 16:
+        raise ValueError("out must be a contiguous, 16-byte aligned [B,Hq,Dv] tensor of q's dtype and device")
     if lse is None:
-        lse = torch.empty(B, hq, dtype=torch.float32, device=q.device) if return_lse else None
-    elif lse.shape != (B, hq) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
+        if return_lse:
+            lse = torch.empty((B, hq), dtype=torch.float32, device=device)
+    elif lse.shape != (B, hq) or lse.dtype != torch.float32 or lse.device != device or not lse.is_contiguous():
         raise ValueError("lse must be a contiguous float32 [B,Hq] tensor on q's device")
-    lib, code = _lib.load(), _dtype_code(q)
-    with _on_device_of(q):
-        need = lib.nsa_dense_decode_workspace_bytes(B, hq, cache.hkv, dk, cache.dv, cache.ctx_cap, sliding_window, code)
-        # a workspace of this call's own: two captured graphs, or two streams, never share one
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-        rc = lib.nsa_dense_decode_step(
-            _ptr(q), _ptr(k_c), _ptr(v_c), _ptr(cache.block_table) if paged else None, cache.max_pages if paged else 0,
-            cache.num_pages if paged else 0, _ptr(cache.ctx_lens), _ptr(out), _ptr(lse), B, hq, cache.hkv, dk, cache.dv,
-            cache.ctx_cap, sliding_window, float(scale), code, _ptr(ws), max(need, 0), _stream())
-    _lib.check(rc, "nsa_dense_decode_step")
+    code = _dtype_code(q)
+    need = _dense_workspace_bytes(B, hq, hkv, dk, dv, cache.ctx_cap, sliding_window, code)
+    # a workspace of this call's own: two captured graphs, or two streams, never share one
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+    rc = _lib.load().nsa_dense_decode_step(
+        q.data_ptr(), k_c.data_ptr(), v_c.data_ptr(), cache.block_table.data_ptr() if paged else None,
+        cache.max_pages if paged else 0, cache.num_pages if paged else 0, cache.ctx_lens.data_ptr(), out.data_ptr(),
+        None if lse is None else lse.data_ptr(), B, hq, hkv, dk, dv, cache.ctx_cap, sliding_window, scale, code,
+        None if ws is None else ws.data_ptr(), need, _raw_stream(device))
+    if rc:
+        _lib.check(rc, "nsa_dense_decode_step")
     return (out, lse) if return_lse else out
 
 

@@ -2,7 +2,6 @@
 enqueue the kernels on the current stream.  No arithmetic happens in Python."""
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import math
 import os
@@ -37,11 +36,9 @@ def _need_cuda(*ts):
             raise RuntimeError("NSA kernels run on the GPU only; got a %s tensor" % t.device)
 
 
-def _on_device_of(t: torch.Tensor):
-    """Makes t's GPU the current one for a launch, so that the current stream is one of that GPU."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _raw_stream(device: torch.device) -> int:
+    """hipStream_t of the device's current stream, without the Stream object that _stream() builds (about 1 us)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _dense(t: torch.Tensor) -> torch.Tensor:
