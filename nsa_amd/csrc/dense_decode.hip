@@ -19,7 +19,9 @@
 
 namespace nsa {
 
-constexpr int kDenseWaves = 4;
+constexpr int kDenseWaves = 4;         // wavefronts of a workgroup that shares a sequence with others
+constexpr int kDenseWholeWaves = 8;    // and of one that takes a whole (short) sequence
+constexpr int kDenseWholePages = 16;
 constexpr int kDenseMinPages = 2;      // fewest pages per unit: one 32-key chunk for each wavefront
 
 struct DenseSpan { int n, lo, first, pages; };   // tokens, first visible token, its page, pages to read
@@ -152,17 +154,18 @@ __device__ __forceinline__ void dense_values(DecState<T, DK, DV> (&st)[NT], vec8
 // Registers (32-bit, per lane) of one chunk's fragments, of the queries and sums of NT head tiles, and what else there is.
 template <typename T, int DK, int DV, int NT> constexpr int kDenseRegs =
     (2 * (DK / 32) + DV / 16) * 2 * (int)sizeof(T) + NT * ((DK / 32) * 2 * (int)sizeof(T) + DV / 4) + 48;
-// Wavefronts per SIMD that the register file (512) then holds.
-template <typename T, int DK, int DV, int NT> constexpr int kDenseOccupancy =
-    kDenseRegs<T, DK, DV, NT> <= 128 ? 4 : kDenseRegs<T, DK, DV, NT> <= 168 ? 3 : kDenseRegs<T, DK, DV, NT> <= 256 ? 2 : 1;
+// Wavefronts per SIMD that the register file (512) then holds, of W of a workgroup at least.
+template <typename T, int DK, int DV, int NT, int W> constexpr int kDenseOccupancy =
+    kDenseRegs<T, DK, DV, NT> <= 128 ? 4 : kDenseRegs<T, DK, DV, NT> <= 168 ? 3 :
+    kDenseRegs<T, DK, DV, NT> <= 256 || W > 4 ? 2 : 1;
 
 // NT: 16-head tiles of the GQA group that share the loaded keys and values.  grid: unit * (hkv * head blocks) + those
-template <typename T, int DK, int DV, int NT>
-__global__ void __launch_bounds__(kDenseWaves * 64, (kDenseOccupancy<T, DK, DV, NT>))
+template <typename T, int DK, int DV, int NT, int W>
+__global__ void __launch_bounds__(W * 64, (kDenseOccupancy<T, DK, DV, NT, W>))
 dense_decode_kernel(const DenseDecodeArgs a) {
   constexpr int kPitch = DV + 4;
-  __shared__ float plane[kDenseWaves][16][kPitch];
-  __shared__ float ml[kDenseWaves][16][2];
+  __shared__ float plane[W][16][kPitch];
+  __shared__ float ml[W][16][2];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n16 = lane & 15, g = lane >> 4;
   const int G = a.hq / a.hkv, blocks = (G + 16 * NT - 1) / (16 * NT);
@@ -171,8 +174,8 @@ dense_decode_kernel(const DenseDecodeArgs a) {
   const int h = hb / blocks, row0 = (hb % blocks) * 16 * NT;
 
   // the plan: which sequence this unit belongs to, and which of its units it is
-  const int C = dense_unit_pages(a);
-  int b = -1, idx = 0, count = 0, before = 0;
+  int b = a.part == nullptr ? unit : -1, idx = 0, count = 1, before = 0;
+  const int C = a.part == nullptr ? a.ctx_cap : dense_unit_pages(a);
   for (int b0 = 0; b0 < a.batch && b < 0; b0 += 64) {
     const int mine = b0 + lane;
     const int nu = mine < a.batch ? dense_units_of(dense_span(a.ctx_lens[mine], a.ctx_cap, a.window).pages, C) : 0;
@@ -248,7 +251,7 @@ dense_decode_kernel(const DenseDecodeArgs a) {
     while (true) {
       float s[NT][8];
       dense_scores<T, DK, NT>(k0, k1, q, s);
-      const int next = cb + 32 * kDenseWaves;
+      const int next = cb + 32 * W;
       if (next < end) {
         id = paged ? page_of(next) : 0;
         load_keys(next, id);
@@ -271,7 +274,7 @@ dense_decode_kernel(const DenseDecodeArgs a) {
     __syncthreads();
     float M = kNegInf;
 #pragma unroll
-    for (int x = 0; x < kDenseWaves; ++x) M = fmaxf(M, ml[x][n16][0]);
+    for (int x = 0; x < W; ++x) M = fmaxf(M, ml[x][n16][0]);
     const float own = M == kNegInf ? 0.f : fast_exp2(st[j].m - M);
 #pragma unroll
     for (int t = 0; t < DV / 16; ++t) {
@@ -281,15 +284,15 @@ dense_decode_kernel(const DenseDecodeArgs a) {
       *reinterpret_cast<f32x4_t*>(&plane[w][n16][16 * t + 4 * g]) = o;
     }
     __syncthreads();
-    for (int item = threadIdx.x; item < 16 * (DV / 4); item += kDenseWaves * 64) {
+    for (int item = threadIdx.x; item < 16 * (DV / 4); item += W * 64) {
       const int r = item / (DV / 4), d = 4 * (item % (DV / 4));
       if (16 * j + r >= rows) break;
       float Mr = kNegInf, L = 0.f;
 #pragma unroll
-      for (int x = 0; x < kDenseWaves; ++x) Mr = fmaxf(Mr, ml[x][r][0]);
+      for (int x = 0; x < W; ++x) Mr = fmaxf(Mr, ml[x][r][0]);
       f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int x = 0; x < kDenseWaves; ++x) {
+      for (int x = 0; x < W; ++x) {
         if (Mr != kNegInf) L += ml[x][r][1] * fast_exp2(ml[x][r][0] - Mr);
         o += *reinterpret_cast<const f32x4_t*>(&plane[x][r][d]);
       }
@@ -407,7 +410,14 @@ DensePlan dense_decode_plan(const DenseDecodeArgs& a) {
   const long in_flight = 32L * kDenseWaves * (a.dk + a.dv) * (a.dtype == 1 ? 4 : 2);
   const long workgroups = 256 * min(4L, max(1L, 65536 / in_flight));
   p.units = (int)max(1L, min(workgroups / per, (long)a.batch * span));
-  p.split = span > kDenseMinPages;         // otherwise every sequence is one unit
+  // A short capacity is not worth a second launch: 8 wavefronts take the whole sequence.  16 / 4 heads, split against
+  // whole, us: one sequence of 512 tokens, 64 / 64 bf16 9.0, 6.7, of 1024 8.8, 10.3; 128 / 128 bf16
+  // 256 tokens 9.7, 6.7, 512 9.7, 10.3; 64 / 64 fp32 256 tokens 10.1, 6.9, 512 10.1, 11.8.  64 sequences fill the card
+  // without a split: 1024 tokens, 128 / 128 bf16 27.0, 23.4, fp32 54.6, 52.2.
+  const long span_bytes = 64L * span * (a.dk + a.dv) * (a.dtype == 1 ? 4 : 2);
+  p.whole = p.tiles == 1 && (span_bytes <= 200 << 10 || (span <= kDenseWholePages && (long)a.batch * a.hkv >= 256));
+  p.split = !p.whole && span > kDenseMinPages;         // otherwise every sequence is one unit
+  if (!p.split) p.units = a.batch;
   p.slots = ((long)p.units + a.batch) * per;
   p.rows = 16 * p.tiles;
   return p;
@@ -423,7 +433,14 @@ static int launch_dense_n(const DenseDecodeArgs& a, const DensePlan& p, hipStrea
   const long units = p.split ? (long)p.units + a.batch : a.batch;
   const long wgs = units * a.hkv * p.blocks;
   if (wgs > 0x7fffffffL || (long)a.batch * a.hq > 0x7fffffffL) return -5;
-  hipLaunchKernelGGL((dense_decode_kernel<T, DK, DV, NT>), dim3((unsigned)wgs), dim3(kDenseWaves * 64), 0, st, a);
+  if constexpr (NT == 1) {
+    if (p.whole) {
+      hipLaunchKernelGGL((dense_decode_kernel<T, DK, DV, NT, kDenseWholeWaves>), dim3((unsigned)wgs),
+                         dim3(kDenseWholeWaves * 64), 0, st, a);
+      return 0;
+    }
+  }
+  hipLaunchKernelGGL((dense_decode_kernel<T, DK, DV, NT, kDenseWaves>), dim3((unsigned)wgs), dim3(kDenseWaves * 64), 0, st, a);
   if (p.split)
     hipLaunchKernelGGL((dense_decode_join_kernel<T, DV>), dim3((unsigned)(a.batch * a.hq)), dim3(256), 0, st, a, p.rows,
                        p.blocks);
@@ -452,7 +469,7 @@ static int launch_dense(const DenseDecodeArgs& a, const DensePlan& p, hipStream_
 int launch_dense_decode(DenseDecodeArgs a, void* workspace, hipStream_t st) {
   const DensePlan p = dense_decode_plan(a);
   a.units = p.units;
-  a.part = reinterpret_cast<float*>(workspace);
+  a.part = p.split ? reinterpret_cast<float*>(workspace) : nullptr;      // null: every sequence is one unit
   a.part_ml = p.split ? a.part + p.slots * p.rows * a.dv : nullptr;
   if (a.dtype == 0) return launch_dense<bf16_t>(a, p, st);
   if (a.dtype == 2) return launch_dense<f16_t>(a, p, st);

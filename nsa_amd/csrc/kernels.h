@@ -149,7 +149,7 @@ struct DenseDecodeArgs {
   float scale; int dtype;
   int units; float* part; float* part_ml;                  // filled in by the launch
 };
-struct DensePlan { int tiles, blocks, units, rows; long slots; bool split; };
+struct DensePlan { int tiles, blocks, units, rows; long slots; bool whole, split; };
 DensePlan dense_decode_plan(const DenseDecodeArgs& a);
 long dense_decode_workspace_bytes(const DenseDecodeArgs& a);
 int launch_dense_decode(DenseDecodeArgs a, void* workspace, hipStream_t st);
