@@ -57,6 +57,7 @@ SIGNATURES = {
     "nsa_decode_split_max_compressed": (_I, []),
     "nsa_decode_step": (_I, [_P] * 9 + [_I] * 15 + [_F, _I, _I, _P]),
     "nsa_qkv_rope": (_I, [_P] * 8 + [_I, _L] + [_I] * 14 + [_P]),
+    "nsa_qkv_rope_axes": (_I, [_P] * 7 + [_I, _P, _L] + [_I] * 14 + [_P]),
     "nsa_decode_append": (_I, [_P] * 7 + [_I] * 9 + [_P]),
     "nsa_decode_step_paged": (_I, [_P] * 4 + [_I] + [_P] * 6 + [_I] * 14 + [_F, _I, _I, _P]),
     "nsa_decode_split_workspace_bytes": (_L, [_I] * 5),

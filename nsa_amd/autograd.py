@@ -224,19 +224,26 @@ class QkvRopeFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, packed, hq, hkv, dk, dv, offsets, inv_freq, positions, cu, rope_off, rope_dim, interleaved,
-                with_gates):
+                with_gates, pair_axis=None):
         ctx.rows, ctx.like = packed.shape[0], (packed.dtype, packed.device)
-        ctx.meta = (packed.shape[1], offsets, inv_freq, positions, cu, rope_off, rope_dim, interleaved, with_gates,
-                    (hq, hkv, dk, dv))
+        kept = (inv_freq, positions)
+        if pair_axis is not None:        # position buffers get reused: a change before the backward has to be noticed
+            ctx.save_for_backward(*kept)
+            kept = (None, None)
+        ctx.meta = (packed.shape[1], offsets, *kept, cu, rope_off, rope_dim, interleaved, with_gates,
+                    (hq, hkv, dk, dv), pair_axis)
         q, k, v, g = ops.qkv_rope_split(packed, hq, hkv, dk, dv, offsets, inv_freq, positions, cu, rope_off, rope_dim,
-                                        interleaved, with_gates)
+                                        interleaved, with_gates, pair_axis)
         if g is None:
             return q, k, v
         return q, k, v, g
 
     @staticmethod
     def backward(ctx, dq, dk_, dv_, dg=None):
-        ld, offsets, inv_freq, positions, cu, rope_off, rope_dim, interleaved, with_gates, (hq, hkv, dk, dv) = ctx.meta
+        ld, offsets, inv_freq, positions, cu, rope_off, rope_dim, interleaved, with_gates, (hq, hkv, dk, dv), pair_axis = \
+            ctx.meta
+        if pair_axis is not None:
+            inv_freq, positions = ctx.saved_tensors
 
         def dense(g, heads, dim):
             if g is not None:
@@ -247,5 +254,5 @@ class QkvRopeFn(torch.autograd.Function):
         if with_gates:
             dg = dense(dg, hq, 3)
         d_packed = ops.qkv_rope_pack(dq, dk_, dv_, dg if with_gates else None, ld, offsets, inv_freq, positions, cu,
-                                     rope_off, rope_dim, interleaved)
-        return (d_packed,) + (None,) * 12
+                                     rope_off, rope_dim, interleaved, pair_axis)
+        return (d_packed,) + (None,) * 13

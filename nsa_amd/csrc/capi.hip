@@ -323,6 +323,45 @@ int nsa_qkv_rope(void* packed, void* q, void* k, void* v, void* gates, const flo
   return finish(rc, "qkv_rope");
 }
 
+int nsa_qkv_rope_axes(void* packed, void* q, void* k, void* v, void* gates, const float* inv_freq,
+                      const int32_t* positions, int axes, const int32_t* pair_axis, int64_t total, int ld, int q_off,
+                      int k_off, int v_off, int g_off, int hq, int hkv, int dk, int dv, int rope_off, int rope_dim,
+                      int interleaved, int pack, int dtype, nsa_stream_t stream) {
+  if (!packed || !q || !k || !v || !inv_freq || !positions || !pair_axis)
+    return fail(NSA_ERR_INVALID, "qkv_rope_axes: null pointer");
+  if (!dtype_ok(dtype)) return fail(NSA_ERR_INVALID, "qkv_rope_axes: bad dtype");
+  if (total <= 0 || hq <= 0 || hkv <= 0 || dk <= 0 || dv <= 0 || dk % 8 != 0 || dv % 8 != 0)
+    return fail(NSA_ERR_INVALID, "qkv_rope_axes: sizes must be positive and head dims multiples of 8");
+  const int64_t nq = (int64_t)hq * dk, nk = (int64_t)hkv * dk, nv = (int64_t)hkv * dv, ng = 3 * (int64_t)hq;
+  if (ld % 8 != 0 || q_off % 8 != 0 || k_off % 8 != 0 || v_off % 8 != 0 || q_off < 0 || k_off < 0 || v_off < 0 ||
+      q_off + nq > ld || k_off + nk > ld || v_off + nv > ld)
+    return fail(NSA_ERR_INVALID, "qkv_rope_axes: column offsets and row stride must be multiples of 8 inside the row");
+  if (gates && (g_off < 0 || g_off + ng > ld)) return fail(NSA_ERR_INVALID, "qkv_rope_axes: gate columns outside the row");
+  if (rope_dim <= 0 || rope_off < 0 || rope_off % 8 != 0 || rope_off > dk - rope_dim ||
+      rope_dim % (interleaved ? 8 : 16) != 0)
+    return fail(NSA_ERR_INVALID, "qkv_rope_axes: rotary channels must be an 8-aligned range inside the head "
+                                 "(length a multiple of 16, or of 8 when interleaved)");
+  if (rope_dim > 256) return fail(NSA_ERR_UNSUPPORTED, "qkv_rope_axes: more than 256 rotary channels");
+  if (axes < 1 || axes > 4) return fail(NSA_ERR_INVALID, "qkv_rope_axes: 1 to 4 axes");
+  nsa::RopeAxesArgs a{};
+  for (int i = 0; i < rope_dim / 2; ++i) {
+    if (pair_axis[i] < 0 || pair_axis[i] >= axes) return fail(NSA_ERR_INVALID, "qkv_rope_axes: pair %d names axis %d of %d", i, pair_axis[i], axes);
+    a.pair_axis[i >> 4] |= (unsigned)pair_axis[i] << (2 * (i & 15));
+  }
+  if (!aligned16(packed) || !aligned16(q) || !aligned16(k) || !aligned16(v))
+    return fail(NSA_ERR_INVALID, "qkv_rope_axes: pointers must be 16-byte aligned");
+  a.base = nsa::QkvRopeArgs{packed, q, k, v, gates, inv_freq, positions, nullptr, 0, (long)total, ld, q_off, k_off, v_off,
+                            g_off, hq, hkv, dk, dv, rope_off, rope_dim, interleaved ? 1 : 0, pack ? 1 : 0, dtype};
+  int64_t end = q_off + nq;
+  if (k_off + nk > end) end = k_off + nk;
+  if (v_off + nv > end) end = v_off + nv;
+  if (gates && g_off + ng > end) end = g_off + ng;
+  a.pad_off = (int)end;
+  const int rc = nsa::launch_rope_axes(a, stream);
+  if (rc == -2) return fail(NSA_ERR_UNSUPPORTED, "qkv_rope_axes: more than 2^31-1 rows or workgroups, or 480000 elements in a row");
+  return finish(rc, "qkv_rope_axes");
+}
+
 int nsa_gate_fwd(const void* q, const void* weight, const void* bias, void* gates, int64_t rows, int dim, int dtype,
                  nsa_stream_t stream) {
   if (!q || !weight || !gates) return fail(NSA_ERR_INVALID, "gate: null pointer");

@@ -165,6 +165,14 @@ struct QkvRopeArgs {
   long total; int ld, q_off, k_off, v_off, g_off, hq, hkv, dk, dv, rope_off, rope_dim, interleaved, pack, dtype;
 };
 int launch_qkv_rope(const QkvRopeArgs& a, hipStream_t st);
+// The same with positions [axes][total]: pair i turns by positions[axis of pair i]; two bits per pair name the axis.
+struct RopeAxesArgs {
+  QkvRopeArgs base;
+  unsigned pair_axis[8];
+  int pad_off;                                             // pack: columns [pad_off, ld) of a row are cleared
+  unsigned pieces, magic; bool small;                      // filled in by the launch
+};
+int launch_rope_axes(RopeAxesArgs a, hipStream_t st);
 
 int launch_compress(const CompressArgs& a, hipStream_t st);
 int launch_compress_bwd(const CompressBwdArgs& a, hipStream_t st);

@@ -14,7 +14,7 @@ Parameter names follow the common decoder-layer convention (`q_proj`, `k_proj`, 
 from __future__ import annotations
 
 import math
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 from torch import nn
@@ -30,19 +30,39 @@ def _round_up(x: int, m: int) -> int:
     return (x + m - 1) // m * m
 
 
+def rope_pair_axes(pairs_per_axis, layout: str = "blocks"):
+    """The axis of every rotary pair, one entry per pair: "blocks" gives the first pairs_per_axis[0] pairs to axis 0, the
+    next ones to axis 1 and so on; "turns" deals them out in turn (0, 1, 2, 0, 1, 2, ...) until an axis has its number."""
+    counts = [int(n) for n in pairs_per_axis]
+    if not 1 <= len(counts) <= 4 or min(counts) < 0:
+        raise ValueError("1 to 4 axes, each with a number of pairs")
+    if layout == "blocks":
+        return tuple(a for a, n in enumerate(counts) for _ in range(n))
+    if layout != "turns":
+        raise ValueError("layout in {'blocks','turns'}")
+    return tuple(a for i in range(max(counts)) for a, n in enumerate(counts) if i < n)
+
+
 class NSAAttentionLayer(nn.Module):
     """hidden_states -> attention output of the same shape.
 
     qk_head_dim / v_head_dim: head sizes of q,k and of v (e.g. 192 / 128); rope_dim: how many
     trailing channels of every q and k head are rotary (192 = 128 content + 64 rotary); 0 = none.
-    rope_interleaved pairs channels (2i, 2i+1) instead of (i, i + rope_dim/2)."""
+    rope_interleaved pairs channels (2i, 2i+1) instead of (i, i + rope_dim/2).
+
+    rope_axes: positions on several axes, e.g. time, height and width of a picture's or film's tokens: how many of the
+    rope_dim/2 pairs follow each axis (up to four), dealt out by rope_axes_layout ("blocks" | "turns", see
+    rope_pair_axes).  rope_axes_spectrum "shared": pair i keeps the frequency it has without axes; "own": the pairs of
+    every axis run through the whole spectrum by themselves.  forward() then takes position_ids [axes, B, T] (or
+    [axes, total] for packed rows); without them a token has its place in the sequence on every axis, as text does."""
 
     def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, qk_head_dim: int = 128,
                  v_head_dim: Optional[int] = None, rope_dim: int = 0, rope_theta: float = 10000.0,
                  rope_interleaved: bool = False, bias: bool = False, compression_stride: int = 16,
                  compression_block: int = 32, selection_block: int = 64, selected_block_count: int = 16,
                  sliding_window: int = 512, compressor_mode: str = "conv", gate_activation: Optional[str] = None,
-                 softmax_scale: Optional[float] = None, device=None, dtype=None):
+                 softmax_scale: Optional[float] = None, device=None, dtype=None, rope_axes: Optional[Sequence[int]] = None,
+                 rope_axes_layout: str = "blocks", rope_axes_spectrum: str = "shared"):
         super().__init__()
         v_head_dim = qk_head_dim if v_head_dim is None else v_head_dim
         if num_heads % num_kv_heads != 0:
@@ -67,6 +87,20 @@ class NSAAttentionLayer(nn.Module):
             inv = 1.0 / (rope_theta ** (torch.arange(0, rope_dim, 2, dtype=torch.float32, device=device) / rope_dim))
         else:
             inv = None
+        self.pair_axis = None
+        if rope_axes is not None:
+            if not rope_dim or sum(rope_axes) * 2 != rope_dim:
+                raise ValueError("rope_axes must share out the %d rotary pairs, got %s" % (rope_dim // 2, tuple(rope_axes)))
+            if rope_axes_spectrum not in ("shared", "own"):
+                raise ValueError("rope_axes_spectrum in {'shared','own'}")
+            self.pair_axis = rope_pair_axes(rope_axes, rope_axes_layout)
+            self.n_axes = len(rope_axes)
+            if rope_axes_spectrum == "own":
+                seen, place = [0] * self.n_axes, []
+                for a in self.pair_axis:
+                    place.append(seen[a] / rope_axes[a])
+                    seen[a] += 1
+                inv = 1.0 / (rope_theta ** torch.tensor(place, dtype=torch.float32, device=device))
         self.register_buffer("inv_freq", inv, persistent=False)
         # packed row of the fused projection: [q | k | v | gate logits | padding to a multiple of 8]
         nq, nk, nv = num_heads * qk_head_dim, num_kv_heads * qk_head_dim, num_kv_heads * v_head_dim
@@ -140,18 +174,23 @@ class NSAAttentionLayer(nn.Module):
                 max_seqlen = int((cu_seqlens[1:] - cu_seqlens[:-1]).max())
         cache = past_key_value
         if cache is not None and T == 1:
-            return self._decode(x, cache).view(shape), None
+            return self._decode(x, cache, position_ids).view(shape), None
         train = needs_grad(x, *self.parameters())
         weight, bias = self.fused_projection() if train else self._fused_cached()
-        positions = None if position_ids is None else position_ids.reshape(-1).to(torch.int32)
+        if self.pair_axis is not None:
+            positions = self._axis_positions(position_ids, x.shape[0], cu_seqlens)
+        else:
+            positions = None if position_ids is None else position_ids.reshape(-1).to(torch.int32)
         rope = (self.inv_freq, positions, cu_seqlens, self.dk - self.rope_dim, self.rope_dim, self.rope_interleaved)
         if train:
             packed = F.linear(x, weight, bias)
-            q, k, v, gates = QkvRopeFn.apply(packed, self.hq, self.hkv, self.dk, self.dv, self.offsets, *rope, True)
+            q, k, v, gates = QkvRopeFn.apply(packed, self.hq, self.hkv, self.dk, self.dv, self.offsets, *rope, True,
+                                             self.pair_axis)
         else:
             with torch.no_grad():
                 packed = F.linear(x, weight, bias)
-                q, k, v, gates = ops.qkv_rope_split(packed, self.hq, self.hkv, self.dk, self.dv, self.offsets, *rope)
+                q, k, v, gates = ops.qkv_rope_split(packed, self.hq, self.hkv, self.dk, self.dv, self.offsets, *rope,
+                                                    pair_axis=self.pair_axis)
         o = self.attn(q, k, v, cu_seqlens, 0 if uniform_len is not None else max_seqlen, gates=gates,
                       return_indices=return_indices)
         idx = None
@@ -164,17 +203,33 @@ class NSAAttentionLayer(nn.Module):
         out = self.o_proj(o.reshape(x.shape[0], self.hq * self.dv))
         return out.view(shape), idx
 
+    def _axis_positions(self, position_ids, total, cu_seqlens):
+        """Positions int32 [axes, total]; without position_ids the place inside the sequence on every axis."""
+        if position_ids is None:
+            cu_seqlens = cu_seqlens.to(torch.int32)
+            rows = torch.arange(total, dtype=torch.int32, device=cu_seqlens.device)
+            start = cu_seqlens[torch.searchsorted(cu_seqlens[1:].contiguous(), rows, right=True)]
+            return (rows - start).expand(self.n_axes, -1)
+        if position_ids.shape[0] != self.n_axes or position_ids.numel() != self.n_axes * total:
+            raise ValueError("position_ids must be [%d axes, B, T] (or [%d, total]), got %s"
+                             % (self.n_axes, self.n_axes, tuple(position_ids.shape)))
+        return position_ids.reshape(self.n_axes, total)
+
     @torch.no_grad()
-    def _decode(self, x, cache):
+    def _decode(self, x, cache, position_ids=None):
         if not isinstance(cache, (NSADecodeCache, NSAPagedDecodeCache)):
             raise TypeError("past_key_value must be an NSADecodeCache or NSAPagedDecodeCache")
         if self.attn.compressor.mode != "mean":
             raise NotImplementedError("the decode cache compresses by mean pooling (compressor_mode='mean')")
         weight, bias = self._fused_cached()
         packed = F.linear(x, weight, bias)
+        positions = cache.ctx_lens
+        if self.pair_axis is not None:
+            positions = self._axis_positions(position_ids, x.shape[0], None) if position_ids is not None else \
+                cache.ctx_lens.expand(self.n_axes, -1)
         q, k_new, v_new, gates = ops.qkv_rope_split(
-            packed, self.hq, self.hkv, self.dk, self.dv, self.offsets, self.inv_freq, cache.ctx_lens, None,
-            self.dk - self.rope_dim, self.rope_dim, self.rope_interleaved)
+            packed, self.hq, self.hkv, self.dk, self.dv, self.offsets, self.inv_freq, positions, None,
+            self.dk - self.rope_dim, self.rope_dim, self.rope_interleaved, pair_axis=self.pair_axis)
         cache.append(k_new, v_new)
         a = self.attn
         scale = a.softmax_scale if a.softmax_scale not in (None, True) else 1.0 / math.sqrt(self.dk)
