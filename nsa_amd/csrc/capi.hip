@@ -358,7 +358,7 @@ int nsa_qkv_rope_axes(void* packed, void* q, void* k, void* v, void* gates, cons
   if (gates && g_off + ng > end) end = g_off + ng;
   a.pad_off = (int)end;
   const int rc = nsa::launch_rope_axes(a, stream);
-  if (rc == -2) return fail(NSA_ERR_UNSUPPORTED, "qkv_rope_axes: more than 2^31-1 rows or workgroups, or 480000 elements in a row");
+  if (rc == -2) return fail(NSA_ERR_UNSUPPORTED, "qkv_rope_axes: more than 2^31-1 rows or workgroups");
   return finish(rc, "qkv_rope_axes");
 }
 

@@ -170,7 +170,7 @@ struct RopeAxesArgs {
   QkvRopeArgs base;
   unsigned pair_axis[8];
   int pad_off;                                             // pack: columns [pad_off, ld) of a row are cleared
-  unsigned pieces, magic; bool small;                      // filled in by the launch
+  bool vector_gates; int pieces, cols, side;                                  // filled in by the launch: pieces per row, per workgroup, rows beside each other
 };
 int launch_rope_axes(RopeAxesArgs a, hipStream_t st);
 

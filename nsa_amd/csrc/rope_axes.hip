@@ -5,116 +5,140 @@
 // The angle of a far position is thousands of turns, so it is formed in 64 bits, in turns, and only what is left after
 // the whole turns is rounded to 32 (a product in fp32 is 2e-3 rad off at position 32768).
 //
-// Bound by HBM: every element is read once and written once.  An item is 8 channels of one token; a workgroup takes
-// 256 U consecutive items, across the ends of tokens, so that short rows fill it as well as long ones, with the loads of
-// all U in flight before the first rotation.  The sines of the tokens it touches are computed once, into LDS, while they
-// travel.
+// Bound by HBM: every element is read once and written once.  A piece is 8 channels of a row.  A thread keeps one piece
+// column and walks over U rows, so where a piece lies, whether it rotates and by which pairs is worked out once, and its
+// U loads travel together; a workgroup takes up to 256 neighbouring columns (short rows: several rows side by side).  The
+// sines of the workgroup's rows are computed once, into LDS, while the loads travel.
 #include "common.h"
 #include "kernels.h"
 
 namespace nsa {
 
-constexpr int kRopeItems = 8;      // U of a large call
+// U: 32 bytes per thread in flight.  32768 rows of 64 / 4 heads, 192 / 128 bf16: U = 1 470 us, 2 327 (5.5 TB/s), 3 348,
+// 4 337; 5003 rows of 12 / 4 heads of 128, all rotary, fp32: U = 1 20.8 us, 2 24.1.  Neighbouring workgroups take
+// neighbouring columns of the same rows: 327 us against 386 with neighbouring rows.
+template <typename T> constexpr int kRopeRows = sizeof(T) == 2 ? 2 : 1;
 
 template <typename T, bool PACK, int U>
 __global__ void __launch_bounds__(256)
 rope_axes_kernel(const RopeAxesArgs a) {
-  extern __shared__ float2 turn[];                       // [token of the workgroup][pair]: cosine, sine
+  extern __shared__ float2 turn[];                       // [row of the workgroup][pair]: cosine, sine
   const QkvRopeArgs& r = a.base;
   const int pq = r.hq * r.dk / 8, pk = r.hkv * r.dk / 8, pv = r.hkv * r.dv / 8;
   const int ng = r.gates != nullptr ? 3 * r.hq : 0;
-  const unsigned ppt = a.pieces;
-  const long first = (long)blockIdx.x * (256 * U);
-  const long t0 = a.small ? (long)((unsigned)first / ppt) : first / (long)ppt;
-  const unsigned r0 = (unsigned)(first - t0 * ppt);
   const int half = r.rope_dim / 2;
+  const unsigned slices = (unsigned)(a.pieces + a.cols - 1) / (unsigned)a.cols;
+  const unsigned block = blockIdx.x / slices, col0 = (blockIdx.x - block * slices) * a.cols;
+  const int side = threadIdx.x / a.cols;                 // row beside row 0 of a pass
+  const int p = (int)col0 + (int)(threadIdx.x - side * a.cols);
+  const long t0 = (long)block * (U * a.side) + side;
+  const bool live = side < a.side && p < a.pieces;
 
-  // where item u of this thread reads and writes: 0 nothing, 1 copy, 2 rotate, 3 gate logits
-  int kind[U], chan[U], tok[U];
-  const T* src[U];
-  T* dst[U];
+  // 0 nothing, 1 copy, 2 rotate, 3 gate logits and padding
+  int kind = 0, chan = 0;
+  const T* src = nullptr;
+  T* dst = nullptr;
+  long sstep = 0, dstep = 0;                             // elements from one row to the next
+  const int pg = a.vector_gates ? ng / 8 : 0;            // gate columns that are pieces like the others
+  if (live && p < pq + pk + pv + pg) {
+    T* split;
+    int c, dim, poff;
+    long row;
+    bool rot = true;
+    if (p < pq) { split = reinterpret_cast<T*>(r.q); row = (long)r.hq * r.dk; c = 8 * p; dim = r.dk; poff = r.q_off; }
+    else if (p < pq + pk) { split = reinterpret_cast<T*>(r.k); row = (long)r.hkv * r.dk; c = 8 * (p - pq); dim = r.dk; poff = r.k_off; }
+    else if (p < pq + pk + pv) { split = reinterpret_cast<T*>(r.v); row = (long)r.hkv * r.dv; c = 8 * (p - pq - pk); dim = r.dv; poff = r.v_off; rot = false; }
+    else { split = reinterpret_cast<T*>(r.gates); row = ng; c = 8 * (p - pq - pk - pv); dim = ng; poff = r.g_off; rot = false; }
+    T* packed = reinterpret_cast<T*>(r.packed) + poff + c;
+    split += c;
+    src = PACK ? split : packed;
+    dst = PACK ? packed : split;
+    sstep = PACK ? row : r.ld;
+    dstep = PACK ? r.ld : row;
+    chan = c % dim - r.rope_off;                         // first rotary channel of this piece (multiple of 8)
+    kind = rot && chan >= 0 && chan < r.rope_dim ? 2 : 1;
+  } else if (live) {
+    kind = 3;
+    chan = 8 * (p - pq - pk - pv);
+  }
+  const bool lower = chan < half;
+  const long partner = lower ? half : -half;             // the other channel of a pair, when they are half a range apart
+
   vec8_t<T> x[U], xp[U];
+  if (kind == 1 || kind == 2) {
+    const T* s = src + t0 * sstep;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const unsigned at = r0 + 256 * u + threadIdx.x;
-    tok[u] = (int)__umulhi(at, a.magic);                 // at / ppt, exact: at * ppt < 2^32
-    const int p = (int)(at - tok[u] * ppt);
-    const long t = t0 + tok[u];
-    kind[u] = 0; chan[u] = 0;
-    src[u] = nullptr; dst[u] = nullptr;
-    x[u] = zero8<T>(); xp[u] = zero8<T>();
-    if (t >= r.total) continue;
-    T* prow = reinterpret_cast<T*>(r.packed) + t * r.ld;
-    if (p < pq + pk + pv) {
-      T* split;
-      int c, dim, poff;
-      bool rot = true;
-      if (p < pq) { split = reinterpret_cast<T*>(r.q) + t * r.hq * r.dk; c = 8 * p; dim = r.dk; poff = r.q_off; }
-      else if (p < pq + pk) { split = reinterpret_cast<T*>(r.k) + t * r.hkv * r.dk; c = 8 * (p - pq); dim = r.dk; poff = r.k_off; }
-      else { split = reinterpret_cast<T*>(r.v) + t * r.hkv * r.dv; c = 8 * (p - pq - pk); dim = r.dv; poff = r.v_off; rot = false; }
-      src[u] = PACK ? split + c : prow + poff + c;
-      dst[u] = PACK ? prow + poff + c : split + c;
-      x[u] = load8(src[u]);
-      chan[u] = c % dim - r.rope_off;                    // first rotary channel of this piece (multiple of 8)
-      kind[u] = rot && chan[u] >= 0 && chan[u] < r.rope_dim ? 2 : 1;
-      if (kind[u] == 2 && !r.interleaved) xp[u] = load8(src[u] + (chan[u] < half ? half : -half));
-    } else {
-      kind[u] = 3;
-      chan[u] = 8 * (p - pq - pk - pv);
-    }
-  }
-
-  const int tokens = (int)__umulhi(r0 + 256 * U - 1, a.magic) + 1;
-  for (int i = threadIdx.x; i < tokens * half; i += 256) {
-    const int k = i / half, pair = i - k * half;
-    const long t = t0 + k;
-    if (t < r.total) {
-      const int axis = (a.pair_axis[pair >> 4] >> (2 * (pair & 15))) & 3;
-      const double turns = (double)r.positions[axis * r.total + t] * ((double)r.inv_freq[pair] * 0.15915494309189535);
-      float s, c;
-      sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-      turn[i] = make_float2(c, PACK ? -s : s);
-    }
-  }
-  __syncthreads();
-
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (kind[u] == 0) continue;
-    if (kind[u] == 1) {
-      store8(dst[u], x[u]);
-    } else if (kind[u] == 2) {
-      const float2* cs = turn + tok[u] * half;
-      float y[8];
-      if (r.interleaved) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 w = cs[chan[u] / 2 + i];
-          const float x0 = (float)x[u][2 * i], x1 = (float)x[u][2 * i + 1];
-          y[2 * i] = x0 * w.x - x1 * w.y;
-          y[2 * i + 1] = x1 * w.x + x0 * w.y;
-        }
-      } else {
-        const bool lower = chan[u] < half;
-        const int f0 = lower ? chan[u] : chan[u] - half;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float2 w = cs[f0 + e];
-          y[e] = (float)x[u][e] * w.x + (float)xp[u][e] * (lower ? -w.y : w.y);
-        }
+    for (int u = 0; u < U; ++u) {
+      if (t0 + u * a.side < r.total) {
+        x[u] = load8(s);
+        if (kind == 2 && !r.interleaved) xp[u] = load8(s + partner);
       }
-      store8(dst[u], pack8<T>(y));
-    } else {                                             // gate logits, then the padding of a packed row
-      const long t = t0 + tok[u];
+      s += a.side * sstep;
+    }
+  }
+
+  if ((int)col0 < pq + pk) {                   // columns behind q and k have nothing to rotate
+    const long w0 = (long)block * (U * a.side);
+    for (int i = threadIdx.x; i < U * a.side * half; i += blockDim.x) {
+      const int k = i / half, pair = i - k * half;
+      const long t = w0 + k;
+      if (t < r.total) {
+        const int axis = (a.pair_axis[pair >> 4] >> (2 * (pair & 15))) & 3;
+        const double turns = (double)r.positions[axis * r.total + t] * ((double)r.inv_freq[pair] * 0.15915494309189535);
+        float s, c;
+        sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+        turn[i] = make_float2(c, PACK ? -s : s);
+      }
+    }
+    __syncthreads();
+  }
+
+  if (kind == 1 || kind == 2) {
+    T* d = dst + t0 * dstep;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (t0 + u * a.side >= r.total) break;
+      if (kind == 1) {
+        store8(d, x[u]);
+      } else {
+        const float2* cs = turn + (u * a.side + side) * half;
+        float y[8];
+        if (r.interleaved) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 w = cs[chan / 2 + i];
+            const float x0 = (float)x[u][2 * i], x1 = (float)x[u][2 * i + 1];
+            y[2 * i] = x0 * w.x - x1 * w.y;
+            y[2 * i + 1] = x1 * w.x + x0 * w.y;
+          }
+        } else {
+          cs += lower ? chan : chan - half;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float2 w = cs[e];
+            y[e] = (float)x[u][e] * w.x + (float)xp[u][e] * (lower ? -w.y : w.y);
+          }
+        }
+        store8(d, pack8<T>(y));
+      }
+      d += a.side * dstep;
+    }
+  } else if (kind == 3) {
+    for (int u = 0; u < U; ++u) {
+      const long t = t0 + u * a.side;
+      if (t >= r.total) break;
       T* prow = reinterpret_cast<T*>(r.packed) + t * r.ld;
       T* g = reinterpret_cast<T*>(r.gates) + t * ng;
-      for (int e = chan[u]; e < chan[u] + 8; ++e) {
-        if (e < ng) {
-          if (PACK) prow[r.g_off + e] = g[e];
-          else g[e] = prow[r.g_off + e];
-        } else if (PACK && a.pad_off + (e - ng) < r.ld) {
-          prow[a.pad_off + (e - ng)] = (T)0.0f;
-        }
+      const T* from = PACK ? g : prow + r.g_off;
+      T* to = PACK ? prow + r.g_off : g;
+      T y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (chan + e < ng) y[e] = from[chan + e];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (chan + e < ng) to[chan + e] = y[e];
+        else if (PACK && a.pad_off + (chan + e - ng) < r.ld) prow[a.pad_off + (chan + e - ng)] = (T)0.0f;
       }
     }
   }
@@ -122,21 +146,22 @@ rope_axes_kernel(const RopeAxesArgs a) {
 
 template <typename T, bool PACK, int U>
 static int rope_axes_u(const RopeAxesArgs& a, hipStream_t st) {
-  const long items = a.base.total * a.pieces;
-  const long blocks = (items + 256 * U - 1) / (256 * U);
-  if (blocks > 0x7fffffffL) return -2;
-  const size_t tokens = (256 * U - 1 + a.pieces - 1) / a.pieces + 1;
-  const size_t smem = tokens * (a.base.rope_dim / 2) * sizeof(float2);
-  hipLaunchKernelGGL((rope_axes_kernel<T, PACK, U>), dim3((unsigned)blocks), dim3(256), smem, st, a);
+  const long blocks = (a.base.total + U * a.side - 1) / (U * a.side);
+  const long slices = (a.pieces + a.cols - 1) / a.cols;
+  if (blocks * slices > 0x7fffffffL) return -2;
+  const unsigned threads = (unsigned)(a.cols * a.side + 63) / 64 * 64;
+  const size_t smem = (size_t)U * a.side * (a.base.rope_dim / 2) * sizeof(float2);
+  hipLaunchKernelGGL((rope_axes_kernel<T, PACK, U>), dim3((unsigned)(blocks * slices)), dim3(threads), smem, st, a);
   return 0;
 }
 
 template <typename T>
 static int rope_axes_t(const RopeAxesArgs& a, hipStream_t st) {
-  // few rows: one item per thread, over as many workgroups as there are
-  const bool large = a.base.total * (long)a.pieces >= 256L * 8 * 256;
-  if (a.base.pack) return large ? rope_axes_u<T, true, kRopeItems>(a, st) : rope_axes_u<T, true, 1>(a, st);
-  return large ? rope_axes_u<T, false, kRopeItems>(a, st) : rope_axes_u<T, false, 1>(a, st);
+  // few rows: one per thread, over twice the workgroups (1000 rows of 4 / 1 heads of 64: 4.8 against 6.2 us)
+  constexpr int U = kRopeRows<T>;
+  const bool large = a.base.total * (long)a.pieces >= 1L << 18;
+  if (a.base.pack) return large ? rope_axes_u<T, true, U>(a, st) : rope_axes_u<T, true, 1>(a, st);
+  return large ? rope_axes_u<T, false, U>(a, st) : rope_axes_u<T, false, 1>(a, st);
 }
 
 int launch_rope_axes(RopeAxesArgs a, hipStream_t st) {
@@ -144,10 +169,14 @@ int launch_rope_axes(RopeAxesArgs a, hipStream_t st) {
   const long ng = r.gates != nullptr ? 3L * r.hq : 0;
   const long pad = r.pack ? r.ld - a.pad_off : 0;
   const long pieces = ((long)r.hq * r.dk + (long)r.hkv * (r.dk + r.dv)) / 8 + (ng + pad + 7) / 8;
-  if (pieces > 60000 || r.total > 0x7fffffffL) return -2;
-  a.pieces = (unsigned)pieces;
-  a.magic = (unsigned)((0x100000000ULL + pieces - 1) / pieces);
-  a.small = r.total * pieces + 256 * kRopeItems < 0xffffffffL;
+  if (pieces > 0x7fffffffL / 8 || r.total > 0x7fffffffL) return -2;
+  a.pieces = (int)pieces;
+  a.vector_gates = ng > 0 && ng % 8 == 0 && r.g_off % 8 == 0 && (reinterpret_cast<uintptr_t>(r.gates) & 15) == 0;
+  const int slices = (int)((pieces + 255) / 256);
+  a.cols = (int)((pieces + slices - 1) / slices);
+  a.side = 256 / a.cols;
+  // short rows whose heads have many pairs keep to fewer rows: at most 32 KB of sines
+  while (a.side > 1 && 2 * a.side * (r.rope_dim / 2) * sizeof(float2) > 32768) --a.side;
   if (r.dtype == 2) return rope_axes_t<f16_t>(a, st);
   return r.dtype == 0 ? rope_axes_t<bf16_t>(a, st) : rope_axes_t<float>(a, st);
 }

@@ -723,45 +723,41 @@ def _rope_operands(inv_freq, positions, cu_seqlens, ref):
 
 @functools.lru_cache(maxsize=64)
 def _pair_axis_array(pair_axis):
-    return (C.c_int32 * len(pair_axis))(*pair_axis), max(pair_axis)
+    """The axes as the C array the library reads, and the smallest and the largest of them."""
+    return (C.c_int32 * len(pair_axis))(*pair_axis), min(pair_axis), max(pair_axis)
 
 
 def _qkv_rope_axes(packed, q, k, v, gates, offsets, inv_freq, positions, rope_off, rope_dim, interleaved, pack, pair_axis):
     """The rotation with positions [axes, total] and the axis of every channel pair."""
     total, hq, dk = q.shape
-    hkv, dv = v.shape[1], v.shape[2]
+    _, hkv, dv = v.shape
+    pairs = rope_dim // 2
     if inv_freq is None or positions is None:
         raise ValueError("a rotation on several axes needs inv_freq and positions [axes, total]")
-    pairs = rope_dim // 2
-    if inv_freq.numel() != pairs or len(pair_axis) != pairs:
+    if pairs <= 0 or inv_freq.numel() != pairs or len(pair_axis) != pairs:
         raise ValueError("inv_freq and pair_axis need one entry per pair of rotary channels (%d), got %d and %d"
                          % (pairs, inv_freq.numel(), len(pair_axis)))
     if positions.dim() != 2 or positions.shape[1] != total or not 1 <= positions.shape[0] <= 4:
         raise ValueError("positions must be [axes, total] = [1 to 4, %d], got %s" % (total, tuple(positions.shape)))
     if positions.is_floating_point() or positions.dtype == torch.bool:
         raise TypeError("positions must be whole numbers, got %s" % positions.dtype)
-    axis_of, most = _pair_axis_array(tuple(pair_axis))
-    if most >= positions.shape[0] or min(pair_axis) < 0:
+    axis_of, least, most = _pair_axis_array(tuple(pair_axis))
+    if least < 0 or most >= positions.shape[0]:
         raise ValueError("pair_axis names an axis outside the %d of positions" % positions.shape[0])
-    want = ((q, (total, hq, dk)), (k, (total, hkv, dk)), (v, (total, hkv, dv)), (gates, (total, hq, 3)))
-    for t, shape in want:
-        if t is not None and (t.shape != shape or t.dtype != packed.dtype or t.device != packed.device):
-            raise ValueError("q, k, v and gates must agree in rows, heads, dtype and device: got %s %s on %s where %s %s on "
-                             "%s is due" % (tuple(t.shape), t.dtype, t.device, shape, packed.dtype, packed.device))
     if total == 0:
         return
     dev = packed.device
     inv_freq = inv_freq.to(device=dev, dtype=torch.float32).contiguous()
     positions = positions.to(device=dev, dtype=torch.int32).contiguous()
-    q_off, k_off, v_off, g_off = offsets
-    args = (packed.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), None if gates is None else gates.data_ptr(),
-            inv_freq.data_ptr(), positions.data_ptr(), positions.shape[0], axis_of, total, packed.shape[1], q_off, k_off,
-            v_off, g_off, hq, hkv, dk, dv, rope_off, rope_dim, int(bool(interleaved)), int(pack), _dtype_code(packed))
-    if dev.index == torch.cuda.current_device():
-        rc = _lib.load().nsa_qkv_rope_axes(*args, _raw_stream(dev))
-    else:
+    if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            rc = _lib.load().nsa_qkv_rope_axes(*args, _raw_stream(dev))
+            return _qkv_rope_axes(packed, q, k, v, gates, offsets, inv_freq, positions, rope_off, rope_dim, interleaved,
+                                  pack, pair_axis)
+    q_off, k_off, v_off, g_off = offsets
+    rc = _lib.load().nsa_qkv_rope_axes(
+        packed.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), None if gates is None else gates.data_ptr(),
+        inv_freq.data_ptr(), positions.data_ptr(), positions.shape[0], axis_of, total, packed.shape[1], q_off, k_off,
+        v_off, g_off, hq, hkv, dk, dv, rope_off, rope_dim, bool(interleaved), pack, _dtype_code(packed), _raw_stream(dev))
     if rc:
         _lib.check(rc, "nsa_qkv_rope_axes")
 
@@ -801,6 +797,12 @@ def qkv_rope_pack(dq, dk_, dv_, dgates, ld, offsets, inv_freq=None, positions=No
     dq, dk_, dv_ = _dense(dq), _dense(dk_), _dense(dv_)
     dgates = None if dgates is None else _dense(dgates)
     if pair_axis is not None:
+        total, hq, dk = dq.shape
+        hkv, dv = dv_.shape[1:]
+        for t, shape in ((dk_, (total, hkv, dk)), (dv_, (total, hkv, dv)), (dgates, (total, hq, 3))):
+            if t is not None and (t.shape != shape or t.dtype != dq.dtype or t.device != dq.device):
+                raise ValueError("the gradients must agree in rows, heads, dtype and device: got %s %s on %s where %s %s on "
+                                 "%s is due" % (tuple(t.shape), t.dtype, t.device, shape, dq.dtype, dq.device))
         # the kernel clears what lies behind the last range; a gap before it has to be cleared here
         ends = sorted((o, o + t.shape[1] * t.shape[2]) for o, t in zip(offsets, (dq, dk_, dv_, dgates)) if t is not None)
         gapless = ends[0][0] == 0 and all(a[1] == b[0] for a, b in zip(ends, ends[1:]))
