@@ -471,6 +471,31 @@ int nsa_dense_decode_step(const void* q, const void* k_cache, const void* v_cach
                           int hkv, int dk, int dv, int ctx_cap, int window, float scale, int dtype, void* workspace,
                           int64_t workspace_bytes, nsa_stream_t stream);
 
+/* Forks and moves of whole sequences in the paged cache.  Full pages are shared by reference count; the partly filled last
+ * page of a sequence always has one owner, so appending never writes into a shared page.
+ * nsa_paged_cache_plan is host bookkeeping only and takes HOST pointers throughout: the caller's page table int32
+ * [batch][max_pages] (0 = none), lens [batch] (tokens), held [batch] (pages), refs [num_pages] (slots that hold a page),
+ * free_pages [num_pages] with *n_free entries (a stack; page 0 is never handed out).  Slot slots[i] becomes the first
+ * lengths[i] tokens of what slot parents[i] held before the call, for all i at once (slots[i] == parents[i] shortens a
+ * sequence, length 0 empties it, length -1 is all the parent has).  Returns 0 with the bookkeeping updated and up to 2 n + 2 moves of 5 ints in `moves`;
+ * NSA_ERR_INVALID or NSA_ERR_RESOURCE (not enough free pages) with nothing changed.
+ * nsa_paged_cache_move carries the moves out on the device (`moves` is a HOST pointer, read during the call): page table,
+ * ctx_lens, last pages and compressed rows (block / stride as the cache was built), in one launch per 80 moves.
+ * nsa_paged_cache_compact_plan (host) / nsa_paged_cache_compact_move (device; `pairs`, up to num_pages (page, new page)
+ * pairs, is a HOST pointer): moves pages down until the pages in use are 1 .. *used.  No counterpart in the reference. */
+int nsa_paged_cache_plan(int32_t* table, int32_t* lens, int32_t* held, int32_t* refs, int32_t* free_pages, int32_t* n_free,
+                         int batch, int max_pages, int num_pages, const int32_t* slots, const int32_t* parents,
+                         const int32_t* lengths, int n, int32_t* moves, int32_t* n_moves);
+int nsa_paged_cache_move(void* k_pool, void* v_pool_t, int32_t* block_table, void* ck_cache, void* cv_cache_t,
+                         int32_t* ctx_lens, const int32_t* moves, int n_moves, int batch, int max_pages, int num_pages,
+                         int hkv, int dk, int dv, int nc_cap, int block, int stride, int dtype, nsa_stream_t stream);
+int nsa_paged_cache_compact_plan(int32_t* table, int32_t* lens, int32_t* held, int32_t* refs, int32_t* free_pages,
+                                 int32_t* n_free, int batch, int max_pages, int num_pages, int32_t* pairs,
+                                 int32_t* n_pairs, int32_t* used);
+int nsa_paged_cache_compact_move(void* k_pool, void* v_pool_t, int32_t* block_table, const int32_t* pairs, int n_pairs,
+                                 int batch, int max_pages, int num_pages, int hkv, int dk, int dv, int dtype,
+                                 nsa_stream_t stream);
+
 /* Appends one token per sequence: k_new [batch][hkv][dk] -> row pos[b] of k_cache, v_new
  * [batch][hkv][dv] -> column pos[b] of v_cache_t, and, when pos[b]+1 completes a compression block,
  * the mean of the last `block` tokens as the next row / column of the compressed caches. */

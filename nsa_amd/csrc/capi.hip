@@ -887,6 +887,106 @@ int nsa_dense_decode_step(const void* q, const void* k_cache, const void* v_cach
   return finish(rc, "dense_decode");
 }
 
+static int paged_books(const char* what, nsa::PagedBooks* bk, int32_t* table, int32_t* lens, int32_t* held, int32_t* refs,
+                       int32_t* free_pages, int32_t* n_free, int batch, int max_pages, int num_pages) {
+  if (!table || !lens || !held || !refs || !free_pages || !n_free) return fail(NSA_ERR_INVALID, "%s: null pointer", what);
+  if (batch <= 0 || max_pages <= 0 || num_pages <= 0) return fail(NSA_ERR_INVALID, "%s: sizes must be positive", what);
+  *bk = nsa::PagedBooks{table, lens, held, refs, free_pages, n_free, batch, max_pages, num_pages};
+  return NSA_OK;
+}
+
+int nsa_paged_cache_plan(int32_t* table, int32_t* lens, int32_t* held, int32_t* refs, int32_t* free_pages, int32_t* n_free,
+                         int batch, int max_pages, int num_pages, const int32_t* slots, const int32_t* parents,
+                         const int32_t* lengths, int n, int32_t* moves, int32_t* n_moves) {
+  nsa::PagedBooks bk;
+  const int rc0 = paged_books("paged_cache_plan", &bk, table, lens, held, refs, free_pages, n_free, batch, max_pages, num_pages);
+  if (rc0 != NSA_OK) return rc0;
+  if (n < 0 || (n > 0 && (!slots || !parents || !lengths || !moves)) || !n_moves)
+    return fail(NSA_ERR_INVALID, "paged_cache_plan: null pointer");
+  try {
+    const int rc = nsa::paged_plan(bk, slots, parents, lengths, n, moves, n_moves);
+    if (rc == -1) return fail(NSA_ERR_INVALID, "paged_cache_plan: slots must be different slots of the cache, parents slots of the "
+                                               "cache, and no length beyond the parent's tokens");
+    if (rc == -3) return fail(NSA_ERR_RESOURCE, "the K/V page pool is exhausted");
+    return rc;
+  } catch (...) {
+    return fail(NSA_ERR_RESOURCE, "paged_cache_plan: out of host memory");
+  }
+}
+
+int nsa_paged_cache_compact_plan(int32_t* table, int32_t* lens, int32_t* held, int32_t* refs, int32_t* free_pages,
+                                 int32_t* n_free, int batch, int max_pages, int num_pages, int32_t* pairs,
+                                 int32_t* n_pairs, int32_t* used) {
+  nsa::PagedBooks bk;
+  const int rc = paged_books("paged_cache_compact_plan", &bk, table, lens, held, refs, free_pages, n_free, batch, max_pages, num_pages);
+  if (rc != NSA_OK) return rc;
+  if (!pairs || !n_pairs || !used) return fail(NSA_ERR_INVALID, "paged_cache_compact_plan: null pointer");
+  try {
+    return nsa::paged_compact_plan(bk, pairs, n_pairs, used);
+  } catch (...) {
+    return fail(NSA_ERR_RESOURCE, "paged_cache_compact_plan: out of host memory");
+  }
+}
+
+static int paged_pools(const char* what, nsa::PagedPools* p, void* k_pool, void* v_pool_t, int num_pages, int hkv, int dk,
+                       int dv, int dtype) {
+  if (!k_pool || !v_pool_t) return fail(NSA_ERR_INVALID, "%s: null pointer", what);
+  if (!dtype_ok(dtype)) return fail(NSA_ERR_INVALID, "%s: bad dtype", what);
+  if (num_pages <= 0 || hkv <= 0 || dk <= 0 || dv <= 0) return fail(NSA_ERR_INVALID, "%s: sizes must be positive", what);
+  if (dk % 8 != 0 || dv % 8 != 0) return fail(NSA_ERR_UNSUPPORTED, "%s: head dims must be multiples of 8", what);
+  if (!aligned16(k_pool) || !aligned16(v_pool_t)) return fail(NSA_ERR_INVALID, "%s: pointers must be 16-byte aligned", what);
+  const int64_t elem = dtype == NSA_F32 ? 4 : 2;
+  *p = nsa::PagedPools{k_pool, v_pool_t, (long)(64 * elem * hkv * dk / 16), (long)(64 * elem * hkv * dv / 16)};
+  return NSA_OK;
+}
+
+int nsa_paged_cache_move(void* k_pool, void* v_pool_t, int32_t* block_table, void* ck_cache, void* cv_cache_t,
+                         int32_t* ctx_lens, const int32_t* moves, int n_moves, int batch, int max_pages, int num_pages,
+                         int hkv, int dk, int dv, int nc_cap, int block, int stride, int dtype, nsa_stream_t stream) {
+  nsa::PagedMoveArgs a{};
+  const int rc = paged_pools("paged_cache_move", &a.pools, k_pool, v_pool_t, num_pages, hkv, dk, dv, dtype);
+  if (rc != NSA_OK) return rc;
+  if (!block_table || !ck_cache || !cv_cache_t || !ctx_lens || (n_moves > 0 && !moves))
+    return fail(NSA_ERR_INVALID, "paged_cache_move: null pointer");
+  if (n_moves < 0 || batch <= 0 || max_pages <= 0 || max_pages > 0x7fffffff / 64 || nc_cap <= 0 || nc_cap % 64 != 0 ||
+      block <= 0 || stride <= 0)
+    return fail(NSA_ERR_INVALID, "paged_cache_move: sizes must be positive and nc_cap a multiple of 64");
+  if (!aligned16(ck_cache) || !aligned16(cv_cache_t)) return fail(NSA_ERR_INVALID, "paged_cache_move: pointers must be 16-byte aligned");
+  bool kept = false;                     // whether the register holds a slot
+  for (int i = 0; i < n_moves; ++i) {
+    const int32_t* m = moves + 5L * i;
+    if (m[0] < -1 || m[0] >= batch || m[1] < -1 || m[1] >= batch || m[2] < 0 || m[2] > max_pages * 64 || m[3] < 0 ||
+        m[3] >= num_pages || m[4] < 0 || m[4] >= num_pages || (m[1] < 0 && (kept || m[0] < 0)) || (m[0] < 0 && !kept))
+      return fail(NSA_ERR_INVALID, "paged_cache_move: move %d names a slot, length or page outside the cache", i);
+    if (m[1] < 0) kept = true;
+    else if (m[0] < 0) kept = false;
+  }
+  if (n_moves == 0) return NSA_OK;
+  a.block_table = block_table; a.ck = ck_cache; a.cv = cv_cache_t; a.ctx_lens = ctx_lens;
+  a.max_pages = max_pages; a.hkv = hkv; a.dk = dk; a.dv = dv; a.nc_cap = nc_cap;
+  const int rc2 = nsa::launch_paged_move(a, moves, n_moves, block, stride, dtype == NSA_F32 ? 4 : 2, stream);
+  if (rc2 == -2) return fail(NSA_ERR_UNSUPPORTED, "paged_cache_move: more than 2^31-1 workgroups");
+  return finish(rc2, "paged_cache_move");
+}
+
+int nsa_paged_cache_compact_move(void* k_pool, void* v_pool_t, int32_t* block_table, const int32_t* pairs, int n_pairs,
+                                 int batch, int max_pages, int num_pages, int hkv, int dk, int dv, int dtype,
+                                 nsa_stream_t stream) {
+  nsa::PagedCompactArgs a{};
+  const int rc = paged_pools("paged_cache_compact_move", &a.pools, k_pool, v_pool_t, num_pages, hkv, dk, dv, dtype);
+  if (rc != NSA_OK) return rc;
+  if (!block_table || (n_pairs > 0 && !pairs)) return fail(NSA_ERR_INVALID, "paged_cache_compact_move: null pointer");
+  if (n_pairs < 0 || batch <= 0 || max_pages <= 0) return fail(NSA_ERR_INVALID, "paged_cache_compact_move: sizes must be positive");
+  for (int i = 0; i < n_pairs; ++i)
+    if (pairs[2 * i] <= 0 || pairs[2 * i] >= num_pages || pairs[2 * i + 1] <= 0 || pairs[2 * i + 1] >= num_pages)
+      return fail(NSA_ERR_INVALID, "paged_cache_compact_move: pair %d names a page outside the pool", i);
+  a.block_table = block_table;
+  a.entries = (long)batch * max_pages;
+  const int rc2 = nsa::launch_paged_compact(a, pairs, n_pairs, stream);
+  if (rc2 == -2) return fail(NSA_ERR_UNSUPPORTED, "paged_cache_compact_move: more than 2^31-1 workgroups");
+  return finish(rc2, "paged_cache_compact_move");
+}
+
 int nsa_decode_append(const void* k_new, const void* v_new, void* k_cache, void* v_cache_t, void* ck_cache,
                       void* cv_cache_t, const int32_t* pos, int batch, int hkv, int dk, int dv, int ctx_cap, int nc_cap,
                       int block, int stride, int dtype, nsa_stream_t stream) {

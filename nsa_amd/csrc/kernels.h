@@ -154,6 +154,39 @@ DensePlan dense_decode_plan(const DenseDecodeArgs& a);
 long dense_decode_workspace_bytes(const DenseDecodeArgs& a);
 int launch_dense_decode(DenseDecodeArgs a, void* workspace, hipStream_t st);
 
+// Forks and moves in the paged cache (paged_cache.hip).  Host bookkeeping, owned by the caller: the page table, the tokens
+// and pages of every slot, the slots that hold each page, and the stack of free pages.
+struct PagedBooks {
+  int32_t* table; int32_t* lens; int32_t* held; int32_t* refs; int32_t* free_pages; int32_t* n_free;
+  int batch, max_pages, num_pages;
+};
+constexpr int kPagedMoves = 80;        // moves per launch: they travel as kernel arguments, which hold 4 KB
+constexpr int kPagedRound = 8;         // moves whose loads travel together
+constexpr int kPagedCyclePiece = 64;   // moves of a cycle that stay together
+constexpr int kPagedPairs = 384;       // pages per launch of a compaction
+int paged_plan(const PagedBooks& bk, const int32_t* slots, const int32_t* parents, const int32_t* lengths, int n,
+               int32_t* moves, int32_t* n_moves);
+int paged_compact_plan(const PagedBooks& bk, int32_t* pairs, int32_t* n_pairs, int32_t* used);
+struct PagedPools { void* k_pool; void* v_pool; long k_page, v_page; };   // 16-byte vectors per page
+struct PagedMove { int src, dst, len, rows, tail, round; };               // round: moves of the round that starts here
+struct PagedPair { int src, dst; };
+struct PagedMoveArgs {
+  PagedPools pools;
+  int32_t* block_table; void* ck; void* cv; int32_t* ctx_lens;
+  int max_pages, hkv, dk, dv, nc_cap;
+  long ck_blocks, cv_blocks, table_blocks; int rows_most, groups;         // filled in by the launch, as are the lists
+  int group[kPagedMoves + 1];                                             // group g: moves [group[g], group[g + 1])
+  PagedMove moves[kPagedMoves + kPagedRound];
+  PagedPair pairs[kPagedMoves];
+};
+struct PagedCompactArgs {
+  PagedPools pools;
+  int32_t* block_table; long entries; int n_pairs;
+  PagedPair pairs[kPagedPairs];
+};
+int launch_paged_move(PagedMoveArgs a, const int32_t* moves, int n, int block, int stride, int elem, hipStream_t st);
+int launch_paged_compact(PagedCompactArgs a, const int32_t* pairs, int n, hipStream_t st);
+
 // Split of a projection GEMM's packed rows [q | k | v | gate logits] into the attention operands with
 // the rotary embedding applied to q and k (pack == 0), or the reverse gather of their gradients with
 // the inverse rotation (pack == 1).  Column offsets and ld in elements, multiples of 8 except g_off.

@@ -5,6 +5,7 @@ forward over the cached tokens (mean-pool compressor): block importance over eve
 row, top-n blocks, selected + sliding-window + compressed attention, gated sum."""
 from __future__ import annotations
 
+import ctypes as C
 import functools
 import math
 from typing import Optional
@@ -75,6 +76,37 @@ class NSADecodeCache:
         self.ctx_lens += 1
 
 
+class _FreePages:
+    """Stack of free page ids in memory that the library shares; the last entry is handed out first."""
+
+    def __init__(self, num_pages: int):
+        self.ids = (C.c_int32 * max(num_pages, 1))(*range(num_pages - 1, 0, -1))
+        self.n = C.c_int32(max(num_pages - 1, 0))
+
+    def __len__(self):
+        return self.n.value
+
+    def _at(self, i):
+        if not -self.n.value <= i < self.n.value:
+            raise IndexError("free page %d of %d" % (i, self.n.value))
+        return i % self.n.value
+
+    def __getitem__(self, i):
+        return self.ids[self._at(i)]
+
+    def __setitem__(self, i, page):
+        self.ids[self._at(i)] = page
+
+    def pop(self):
+        page = self[-1]
+        self.n.value -= 1
+        return page
+
+    def append(self, page):
+        self.ids[self.n.value] = page
+        self.n.value += 1
+
+
 class NSAPagedDecodeCache:
     """The same caches with K and V in a pool of 64-token pages shared by all sequences (one page =
     one selection block of the default configuration), so that sequences of very different lengths
@@ -83,7 +115,13 @@ class NSAPagedDecodeCache:
     of sequence b; unused entries point at page 0, which is never handed out and stays zero.  The
     compressed caches are small (1/stride of the tokens) and stay contiguous per sequence.
 
-    Page bookkeeping (free list, lengths) lives on the host, so no call here waits for the GPU."""
+    Sequences can share pages: fork() lets one cached sequence continue in several slots (samples of one prompt, a
+    common prefix), reorder() gives every slot the sequence of another one (beam search), truncate() takes tokens back
+    (rejected drafts), compact() moves the pages in use together.  Full pages are shared by reference count; the partly
+    filled last page of a sequence is always its own, so append() never writes into a shared page.
+
+    Page bookkeeping (free list, lengths, counts) lives on the host, so no call here waits for the GPU.  One cache is
+    used by one thread and one stream at a time."""
 
     PAGE = 64
 
@@ -105,27 +143,42 @@ class NSAPagedDecodeCache:
         self.cvt = torch.zeros(batch, hkv, dv, self.nc_cap, **z)
         self.block_table = torch.zeros(batch, self.max_pages, dtype=torch.int32, device=device)
         self.ctx_lens = torch.zeros(batch, dtype=torch.int32, device=device)
-        self._free = list(range(self.num_pages - 1, 0, -1))
-        self._pages = [[] for _ in range(batch)]
-        self._lens = [0] * batch
+        # host bookkeeping, in memory that the library reads and writes: page ids, tokens and pages per slot, and how
+        # many slots hold each page
+        self._free = _FreePages(self.num_pages)
+        self._table = (C.c_int32 * (batch * self.max_pages))()
+        self._lens = (C.c_int32 * batch)()
+        self._held = (C.c_int32 * batch)()
+        self._refs = (C.c_int32 * self.num_pages)()
+        self._shares = False                     # whether any page may be held by more than one slot
 
     @property
     def free_pages(self) -> int:
         return len(self._free)
 
+    def _pages_of(self, b: int):
+        at = b * self.max_pages
+        return self._table[at:at + self._held[b]]
+
+    @property
+    def _pages(self):
+        return [self._pages_of(b) for b in range(self.batch)]
+
     def _grow(self, b: int, new_len: int):
         """Makes sure sequence b owns pages for new_len tokens; returns the (slot, page) pairs added.
         All or nothing: on an error the sequence keeps exactly the pages it had."""
-        need = (new_len + self.PAGE - 1) // self.PAGE
+        need, held = (new_len + self.PAGE - 1) // self.PAGE, self._held[b]
         if need > self.max_pages:
             raise RuntimeError(f"sequence {b} would exceed the cache capacity of {self.ctx_cap} tokens")
-        if need - len(self._pages[b]) > len(self._free):
+        if need - held > len(self._free):
             raise RuntimeError("the K/V page pool is exhausted")
         added = []
-        while len(self._pages[b]) < need:
+        for slot in range(held, need):
             pg = self._free.pop()
-            added.append((len(self._pages[b]), pg))
-            self._pages[b].append(pg)
+            added.append((slot, pg))
+            self._table[b * self.max_pages + slot] = pg
+            self._refs[pg] = 1
+        self._held[b] = max(held, need)
         return added
 
     def _publish(self, entries):
@@ -137,9 +190,15 @@ class NSAPagedDecodeCache:
             e[:, 2].to(device=self.block_table.device, dtype=torch.int32)
 
     def release(self, b: int):
-        """Returns the pages of sequence b to the pool and empties it."""
-        self._free.extend(reversed(self._pages[b]))
-        self._pages[b] = []
+        """Empties sequence b; the pages that no other sequence shares go back to the pool."""
+        at = b * self.max_pages
+        for slot in range(self._held[b] - 1, -1, -1):
+            pg = self._table[at + slot]
+            self._refs[pg] -= 1
+            if self._refs[pg] == 0:
+                self._free.append(pg)
+            self._table[at + slot] = 0
+        self._held[b] = 0
         self._lens[b] = 0
         self.block_table[b].zero_()
         self.ctx_lens[b] = 0
@@ -156,10 +215,20 @@ class NSAPagedDecodeCache:
         B, T = k.shape[:2]
         if B != len(seqs):
             raise ValueError(f"fill() got {B} sequences for {len(seqs)} cache slots")
-        held = sum(len(self._pages[b]) for b in seqs)
+        if self._shares:         # a page goes back only when the last of its holders is refilled
+            holders = {}
+            for b in seqs:
+                for pg in self._pages_of(b):
+                    holders[pg] = holders.get(pg, 0) + 1
+            held = sum(self._refs[pg] == n for pg, n in holders.items())
+        else:
+            held = sum(self._held[b] for b in seqs)
         if len(seqs) * ((T + self.PAGE - 1) // self.PAGE) > len(self._free) + held:
             raise RuntimeError("the K/V page pool is exhausted")       # before any sequence is touched
         entries = []
+        if self._shares:
+            for b in seqs:
+                self.release(b)
         for b in seqs:
             if self._lens[b]:
                 self.release(b)
@@ -168,7 +237,7 @@ class NSAPagedDecodeCache:
         self._publish(entries)
         P, Tp = self.PAGE, _round_up(T, self.PAGE)
         if T > 0:
-            pages = torch.tensor([self._pages[b][:Tp // P] for b in seqs], dtype=torch.int64, device=k.device)
+            pages = torch.tensor([self._pages_of(b)[:Tp // P] for b in seqs], dtype=torch.int64, device=k.device)
             kp = torch.zeros(B, Tp, self.hkv, self.dk, dtype=k.dtype, device=k.device)
             vp = torch.zeros(B, Tp, self.hkv, self.dv, dtype=v.dtype, device=v.device)
             kp[:, :T], vp[:, :T] = k, v
@@ -186,6 +255,97 @@ class NSAPagedDecodeCache:
             self.ck[sq, :nc] = ck.view(B, nc, self.hkv, self.dk)
             self.cvt[sq, :, :, :nc] = cv.view(B, nc, self.hkv, self.dv).permute(0, 2, 3, 1)
         self.ctx_lens[sq] = T
+
+    # -------------------------------------------------------------------------------- forks and moves of sequences
+    def _assign(self, slots, parents, lengths):
+        """Slot slots[i] becomes the first lengths[i] tokens of what slot parents[i] held, for all i at once."""
+        n = len(slots)
+        if n == 0:
+            return
+        device = self.k_pool.device
+        if device.type != "cuda":
+            raise RuntimeError("NSA kernels run on the GPU only; the cache is on %s" % device)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the page bookkeeping lives on the host: forks and moves cannot be captured into a graph")
+        if device.index != torch.cuda.current_device():
+            with torch.cuda.device(device):
+                return self._assign(slots, parents, lengths)
+        if self.dk % 8 or self.dv % 8:
+            raise NotImplementedError("forks and moves take head dims that are multiples of 8")
+        lib, ints, code = _lib.load(), C.c_int32 * n, _dtype_code(self.k_pool)
+        moves, n_moves = (C.c_int32 * (10 * n + 10))(), C.c_int32()
+        rc = lib.nsa_paged_cache_plan(self._table, self._lens, self._held, self._refs, self._free.ids, C.byref(self._free.n),
+                                      self.batch, self.max_pages, self.num_pages, ints(*slots), ints(*parents),
+                                      ints(*lengths), n, moves, C.byref(n_moves))
+        if rc:
+            _lib.check(rc, "nsa_paged_cache_plan")
+        self._shares = True
+        rc = lib.nsa_paged_cache_move(
+            self.k_pool.data_ptr(), self.v_pool_t.data_ptr(), self.block_table.data_ptr(), self.ck.data_ptr(),
+            self.cvt.data_ptr(), self.ctx_lens.data_ptr(), moves, n_moves.value, self.batch, self.max_pages, self.num_pages,
+            self.hkv, self.dk, self.dv, self.nc_cap, self.block, self.stride, code, _raw_stream(device))
+        if rc:
+            _lib.check(rc, "nsa_paged_cache_move")
+
+    def _check_slot(self, b):
+        if not 0 <= b < self.batch:
+            raise ValueError("slot %d of a cache of %d sequences" % (b, self.batch))
+
+    def fork(self, src: int, dst, length: Optional[int] = None):
+        """The sequence of slot src continues in the slots dst (a slot or several) as well, or its first `length` tokens
+        do; what dst held is released.  Full pages are shared, the partly filled last page and the compressed rows are
+        copied, in one launch.  RuntimeError, and nothing changes, when the pool has no pages left for the copies."""
+        dst = [dst] if isinstance(dst, int) else list(dst)
+        self._check_slot(src)
+        length = self._lens[src] if length is None else length
+        if not 0 <= length <= self._lens[src]:
+            raise ValueError("slot %d holds %d tokens, not %d" % (src, self._lens[src], length))
+        if src in dst:
+            raise ValueError("a sequence cannot be forked into its own slot %d" % src)
+        self._assign(dst, [src] * len(dst), [length] * len(dst))
+
+    def reorder(self, parents):
+        """Slot b continues the sequence that slot parents[b] held, for every slot at once, as after a beam-search step; a
+        parent may come up several times or not at all.  Pages are shared and copied as by fork()."""
+        parents = list(parents)
+        if len(parents) != self.batch:
+            raise ValueError("reorder() got %d parents for %d slots" % (len(parents), self.batch))
+        self._check_slot(min(parents))
+        self._check_slot(max(parents))
+        self._assign(range(self.batch), parents, [-1] * self.batch)
+
+    def truncate(self, seq: int, length: int):
+        """Sequence seq keeps its first `length` tokens (a draft that was rejected); the pages behind them go back to the
+        pool.  If the cut falls into a page that other sequences share, the sequence gets a copy of its own."""
+        self._check_slot(seq)
+        if not 0 <= length <= self._lens[seq]:
+            raise ValueError("slot %d holds %d tokens, not %d" % (seq, self._lens[seq], length))
+        self._assign([seq], [seq], [length])
+
+    def compact(self) -> int:
+        """Moves pages until those in use are pages 1 .. n and returns n: k_pool[:n + 1] and v_pool_t[:n + 1] then hold
+        every cached token, e.g. to save them or to carry them over into a smaller pool."""
+        device = self.k_pool.device
+        if device.type != "cuda":
+            raise RuntimeError("NSA kernels run on the GPU only; the cache is on %s" % device)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the page bookkeeping lives on the host: forks and moves cannot be captured into a graph")
+        if device.index != torch.cuda.current_device():
+            with torch.cuda.device(device):
+                return self.compact()
+        if self.dk % 8 or self.dv % 8:
+            raise NotImplementedError("forks and moves take head dims that are multiples of 8")
+        lib, code = _lib.load(), _dtype_code(self.k_pool)
+        pairs, n_pairs, used = (C.c_int32 * (2 * self.num_pages))(), C.c_int32(), C.c_int32()
+        rc = lib.nsa_paged_cache_compact_plan(self._table, self._lens, self._held, self._refs, self._free.ids,
+                                              C.byref(self._free.n), self.batch, self.max_pages, self.num_pages, pairs,
+                                              C.byref(n_pairs), C.byref(used))
+        _lib.check(rc, "nsa_paged_cache_compact_plan")
+        rc = lib.nsa_paged_cache_compact_move(
+            self.k_pool.data_ptr(), self.v_pool_t.data_ptr(), self.block_table.data_ptr(), pairs, n_pairs.value, self.batch,
+            self.max_pages, self.num_pages, self.hkv, self.dk, self.dv, code, _raw_stream(device))
+        _lib.check(rc, "nsa_paged_cache_compact_move")
+        return used.value
 
     def reserve_next(self):
         """Host half of append(): makes sure every sequence owns the page of its next token and

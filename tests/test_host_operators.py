@@ -124,3 +124,294 @@ def test_rope_axes_python_checks(monkeypatch):
     for bad in ((dq, dk[:2], dv, dg), (dq, dk, dv, dg.float()), (dq, dk[:, :, :32].contiguous(), dv, dg)):
         with pytest.raises(ValueError, match="agree"):
             ops.qkv_rope_pack(*bad, 416, args[4], **good)
+
+
+# ------------------------------------------------------------------------------- forks and moves in the paged cache
+
+class Model:
+    """Every slot's tokens as a plain list; the cache's tensors hold token ids (one head, one channel group), its compressed
+    rows the id of their last token."""
+
+    def __init__(self, cache):
+        self.c, self.next = cache, 1
+        self.tokens = [[] for _ in range(cache.batch)]
+
+    def append(self, b, n):
+        c = self.c
+        entries = c._grow(b, c._lens[b] + n)
+        c._publish([(b, s, p) for s, p in entries])
+        for _ in range(n):
+            at = c._lens[b]
+            page = c._pages_of(b)[at // 64]
+            assert c._refs[page] == 1                       # a shared page is never written
+            c.k_pool[page, at % 64] = c.v_pool_t[page, :, :, at % 64] = self.next
+            self.tokens[b].append(self.next)
+            c._lens[b] = at + 1
+            if at + 1 >= c.block and (at + 1 - c.block) % c.stride == 0:
+                row = (at + 1 - c.block) // c.stride
+                c.ck[b, row] = c.cvt[b, :, :, row] = self.next
+            self.next += 1
+        c.ctx_lens[b] = c._lens[b]
+
+    def check(self):
+        c = self.c
+        holders = [0] * c.num_pages
+        for b, want in enumerate(self.tokens):
+            n, pages = len(want), c._pages_of(b)
+            assert c._lens[b] == n and int(c.ctx_lens[b]) == n and len(pages) == (n + 63) // 64
+            assert c.block_table[b].tolist() == pages + [0] * (c.max_pages - len(pages))
+            assert c._table[b * c.max_pages:(b + 1) * c.max_pages] == c.block_table[b].tolist()
+            for p in pages:
+                assert 0 < p < c.num_pages
+                holders[p] += 1
+            if n:
+                ids = torch.tensor(pages)
+                assert c.k_pool[ids].reshape(-1, c.hkv * c.dk)[:n, 0].tolist() == want
+                assert c.v_pool_t[ids].permute(0, 3, 1, 2).reshape(-1, c.hkv * c.dv)[:n, -1].tolist() == want
+            rows = (n - c.block) // c.stride + 1 if n >= c.block else 0
+            last = [want[r * c.stride + c.block - 1] for r in range(rows)]
+            assert c.ck[b, :rows, 0, 0].tolist() == last and c.cvt[b, 0, 0, :rows].tolist() == last
+            if n % 64:
+                assert c._refs[pages[-1]] == 1
+        assert holders == list(c._refs)
+        free = [c._free[i] for i in range(len(c._free))]
+        assert sorted(free) == [p for p in range(1, c.num_pages) if holders[p] == 0]
+
+
+def carry_out(c, moves):
+    """The device half on CPU tensors, in the rounds of the kernel: the loads of a round before its stores."""
+    rows = lambda n: min((n - c.block) // c.stride + 1, c.nc_cap) if n >= c.block else 0     # noqa: E731
+    kept, i = None, 0
+    while i < len(moves):
+        cnt = 1
+        while cnt < 8 and i + cnt < len(moves) and moves[i + cnt][1] >= 0:
+            cnt += 1
+        loaded = [None if m[0] < 0 else (c.ck[m[0]].clone(), c.cvt[m[0]].clone(), c.block_table[m[0]].clone())
+                  for m in moves[i:i + cnt]]
+        for (src, dst, n, tail_src, tail), val in zip(moves[i:i + cnt], loaded):
+            if dst < 0:
+                kept = val
+                continue
+            ck, cvt, table = kept if src < 0 else val
+            if src != dst:
+                c.ck[dst, :rows(n)] = ck[:rows(n)]
+                c.cvt[dst, :, :, :rows(n)] = cvt[:, :, :rows(n)]
+            table = table.clone()
+            table[n // 64:] = 0
+            if n % 64:
+                table[n // 64] = tail
+            c.block_table[dst] = table
+            c.ctx_lens[dst] = n
+        i += cnt
+    for src, dst, n, tail_src, tail in moves:
+        if n % 64 and dst >= 0 and tail_src != tail:
+            c.k_pool[tail], c.v_pool_t[tail] = c.k_pool[tail_src].clone(), c.v_pool_t[tail_src].clone()
+
+
+def plan(lib, c, slots, parents, lengths):
+    n = len(slots)
+    ints = ctypes.c_int32 * max(n, 1)
+    moves, count = (ctypes.c_int32 * (10 * n + 10))(), ctypes.c_int32()
+    rc = lib.nsa_paged_cache_plan(c._table, c._lens, c._held, c._refs, c._free.ids, ctypes.byref(c._free.n), c.batch,
+                                  c.max_pages, c.num_pages, ints(*slots), ints(*parents), ints(*lengths), n, moves,
+                                  ctypes.byref(count))
+    if rc:
+        return rc, None
+    assert count.value <= 2 * n + 2
+    return rc, [tuple(moves[5 * i:5 * i + 5]) for i in range(count.value)]
+
+
+def small_cache(batch, pages, cap=320):
+    from nsa_amd.decode import NSAPagedDecodeCache
+    return NSAPagedDecodeCache(batch, pages, cap, 1, 8, 8, dtype=torch.float32, device="cpu")
+
+
+def books(c):
+    return (list(c._table), list(c._lens), list(c._held), list(c._refs), len(c._free),
+            [c._free[i] for i in range(len(c._free))])
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_paged_moves_against_a_model(lib, seed):
+    """random appends, forks, reorders, cuts and releases: tokens, compressed rows, page table, counts and free list"""
+    import random
+    rng = random.Random(seed)
+    batch = rng.choice([2, 3, 5, 9, 17])
+    c = small_cache(batch, rng.choice([batch * 2, batch * 5]))
+    m = Model(c)
+    refused = 0
+    for _ in range(60):
+        kind = rng.choice(["append", "append", "fork", "reorder", "assign", "truncate", "release"])
+        if kind == "append":
+            b, n = rng.randrange(batch), rng.choice([1, 2, 31, 33, 64, 100])
+            need = (len(m.tokens[b]) + n + 63) // 64
+            if need <= c.max_pages and need - c._held[b] <= len(c._free):
+                m.append(b, n)
+        elif kind == "release":
+            b = rng.randrange(batch)
+            c.release(b)
+            m.tokens[b] = []
+        else:
+            if kind == "fork":
+                src = rng.randrange(batch)
+                slots = rng.sample([b for b in range(batch) if b != src], rng.randint(1, batch - 1))
+                cut = rng.choice([len(m.tokens[src]), rng.randint(0, len(m.tokens[src]))])
+                parents, lengths = [src] * len(slots), [cut] * len(slots)
+            elif kind == "reorder":
+                slots = list(range(batch))
+                parents = rng.sample(slots, batch) if rng.random() < 0.5 else [rng.randrange(batch) for _ in slots]
+                lengths = [rng.choice([-1, len(m.tokens[p])]) for p in parents]
+            elif kind == "assign":
+                slots = rng.sample(range(batch), rng.randint(1, batch))
+                parents = [rng.randrange(batch) for _ in slots]
+                lengths = [rng.randint(0, len(m.tokens[p])) for p in parents]
+            else:
+                slots = parents = [rng.randrange(batch)]
+                lengths = [rng.randint(0, len(m.tokens[slots[0]]))]
+            before = books(c)
+            rc, moves = plan(lib, c, slots, parents, lengths)
+            if rc:
+                assert rc == -3 and books(c) == before
+                refused += 1
+            else:
+                carry_out(c, moves)
+                old = [list(t) for t in m.tokens]
+                for s, p, n in zip(slots, parents, lengths):
+                    m.tokens[s] = old[p][:n] if n >= 0 else list(old[p])
+        m.check()
+    assert refused < 40
+
+
+@pytest.mark.parametrize("n", [2, 3, 62, 63, 64, 65, 66, 130, 200])
+def test_paged_moves_in_cycles_of_any_length(lib, n):
+    """all slots change places in one cycle, in two, and in one with branches"""
+    for pattern in range(3):
+        c = small_cache(n, 4 * n, cap=128)
+        m = Model(c)
+        for b in range(n):
+            m.append(b, 40 + b % 60)
+        order = torch.randperm(n, generator=torch.Generator().manual_seed(n + pattern)).tolist()
+        parents = list(range(n))
+        cut = n if pattern != 1 else max(2, n // 3)
+        for lo, hi in ((0, cut), (cut, n)):
+            ring = order[lo:hi]
+            for i, b in enumerate(ring):
+                parents[b] = ring[(i + 1) % len(ring)]
+        if pattern == 2 and n > 5:
+            parents[order[1]] = order[4]                     # order[2] and order[3] are left with one reader less
+        rc, moves = plan(lib, c, list(range(n)), parents, [len(m.tokens[p]) for p in parents])
+        assert rc == 0
+        # a cycle's piece stays short enough for one launch
+        start = None
+        for i, mv in enumerate(moves):
+            if mv[1] < 0:
+                assert start is None
+                start = i
+            elif mv[0] < 0:
+                assert i - start <= 65
+                start = None
+        assert start is None
+        carry_out(c, moves)
+        old = [list(t) for t in m.tokens]
+        m.tokens = [old[p] for p in parents]
+        m.check()
+
+
+def test_paged_plan_refuses_and_changes_nothing(lib):
+    c = small_cache(4, 4, cap=192)
+    m = Model(c)
+    m.append(0, 100)
+    m.append(1, 70)
+    before = books(c)
+    for slots, parents, lengths in (([4], [0], [0]), ([-1], [0], [0]), ([2], [4], [0]), ([2], [-1], [0]), ([2], [0], [101]),
+                                    ([2], [0], [-2]), ([2, 2], [0, 1], [10, 10])):
+        assert plan(lib, c, slots, parents, lengths)[0] == -1
+        assert books(c) == before
+    assert plan(lib, c, [2, 3], [0, 0], [100, 100])[0] == -3                     # two copies of the last page, none free
+    assert books(c) == before and lib.nsa_last_error_string()
+    m.check()
+    rc, moves = plan(lib, c, [2, 3], [0, 0], [64, 64])                           # whole pages need none
+    carry_out(c, moves)
+    m.tokens[2] = m.tokens[3] = m.tokens[0][:64]
+    m.check()
+    rc, moves = plan(lib, c, [1, 2, 3], [0, 0, 0], [100, 100, 0])                # slot 1's pages become the copies
+    assert rc == 0
+    carry_out(c, moves)
+    m.tokens[1] = m.tokens[2] = m.tokens[0]
+    m.tokens[3] = []
+    m.check()
+    assert plan(lib, c, [], [], [])[0] == 0
+
+
+def test_paged_compaction_plan(lib):
+    c = small_cache(4, 20)
+    m = Model(c)
+    for b in range(4):
+        m.append(b, 130 + b)
+    carry_out(c, plan(lib, c, [3], [2], [128])[1])
+    m.tokens[3] = m.tokens[2][:128]
+    for b in (0, 1):
+        c.release(b)
+        m.tokens[b] = []
+    m.check()
+    pairs, n, used = (ctypes.c_int32 * (2 * c.num_pages))(), ctypes.c_int32(), ctypes.c_int32()
+    args = (c._table, c._lens, c._held, c._refs, c._free.ids, ctypes.byref(c._free.n), c.batch, c.max_pages, c.num_pages,
+            pairs, ctypes.byref(n), ctypes.byref(used))
+    assert lib.nsa_paged_cache_compact_plan(*args) == 0
+    assert used.value == 3 and n.value > 0
+    for i in range(n.value):
+        src, dst = pairs[2 * i], pairs[2 * i + 1]
+        assert src > 3 >= dst
+        c.k_pool[dst], c.v_pool_t[dst] = c.k_pool[src], c.v_pool_t[src]
+        c.block_table[c.block_table == src] = dst
+    m.check()
+    assert [c._free[-1 - i] for i in range(3)] == [4, 5, 6]                      # the lowest free page is handed out first
+    assert lib.nsa_paged_cache_compact_plan(*args) == 0 and n.value == 0 and used.value == 3
+
+
+def test_paged_move_argument_errors_do_not_launch(lib):
+    buf = (ctypes.c_char * 4096)()
+    p = ctypes.addressof(buf) + (-ctypes.addressof(buf)) % 16
+    names = ["k", "v", "table", "ck", "cv", "lens", "moves", "n", "batch", "max_pages", "num_pages", "hkv", "dk", "dv",
+             "nc_cap", "block", "stride", "dtype", "stream"]
+    moves = lambda *a: (ctypes.c_int32 * 40)(*a)                                        # noqa: E731
+    good = dict(k=p, v=p, table=p, ck=p, cv=p, lens=p, moves=moves(0, 1, 70, 1, 2), n=1, batch=2, max_pages=4, num_pages=8,
+                hkv=2, dk=64, dv=64, nc_cap=64, block=32, stride=16, dtype=0, stream=None)
+
+    def call(**kw):
+        return lib.nsa_paged_cache_move(*[dict(good, **kw)[n] for n in names])
+
+    for bad in (dict(k=None), dict(v=None), dict(table=None), dict(ck=None), dict(cv=None), dict(lens=None), dict(moves=None),
+                dict(n=-1), dict(batch=0), dict(max_pages=0), dict(num_pages=0), dict(hkv=0), dict(nc_cap=60), dict(block=0),
+                dict(stride=0), dict(dtype=9), dict(k=p + 8), dict(ck=p + 4),
+                dict(moves=moves(2, 1, 70, 1, 2)), dict(moves=moves(0, 2, 70, 1, 2)), dict(moves=moves(0, 1, 257, 1, 2)),
+                dict(moves=moves(0, 1, -1, 1, 2)), dict(moves=moves(0, 1, 70, 8, 2)), dict(moves=moves(0, 1, 70, 1, -1)),
+                dict(moves=moves(-1, 1, 70, 1, 2)), dict(moves=moves(-1, -1, 70, 1, 2)),
+                dict(moves=moves(0, -1, 70, 1, 2, 1, -1, 70, 1, 2), n=2)):
+        assert call(**bad) == -1, bad
+    assert call(dk=60) == -2 and call(n=0, moves=None) == 0
+    comp = [p, p, p, moves(9, 1), 1, 2, 4, 8, 2, 64, 64, 0, None]
+    assert lib.nsa_paged_cache_compact_move(*comp) == -1
+    comp[3] = moves(3, 0)
+    assert lib.nsa_paged_cache_compact_move(*comp) == -1
+
+
+def test_paged_cache_python_checks():
+    c = small_cache(3, 6)
+    c._publish([(0, s, p) for s, p in c._grow(0, 10)])
+    c._lens[0] = 10
+    for call in (lambda: c.fork(3, 1), lambda: c.fork(-1, 1), lambda: c.fork(0, [0, 1]), lambda: c.fork(0, 1, length=11),
+                 lambda: c.fork(0, 1, length=-1), lambda: c.reorder([0, 1]), lambda: c.reorder([0, 1, 3]),
+                 lambda: c.reorder([0, 1, -1]), lambda: c.truncate(0, 11), lambda: c.truncate(3, 0), lambda: c.truncate(0, -1)):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: c.fork(0, 1), lambda: c.reorder([0, 0, 0]), lambda: c.truncate(0, 5), lambda: c.compact()):
+        with pytest.raises(RuntimeError, match="GPU only"):
+            call()
+    c.fork(0, [])                                                                # nothing to do
+    assert c._lens[0] == 10 and c.free_pages == 5
+    with pytest.raises(IndexError):
+        c._free[5]
+    c.release(0)
+    with pytest.raises(IndexError):
+        [c._free.pop() for _ in range(7)]
