@@ -126,9 +126,20 @@ __device__ __forceinline__ void dense_values(DecState<T, DK, DV> (&st)[NT], vec8
       const float x = s[j][i] * c;
       mx = fmaxf(mx, whole || (key >= lo && key < n) ? x : kNegInf);
     }
-    const float m_new = fmaxf(st[j].m, colgroup_max(mx));
-    const float mref = m_new == kNegInf ? 0.f : m_new;
-    const float alpha = fast_exp2(st[j].m - mref);
+    // The reference of the exponentials follows the maximum only when that has grown by more than 2^8 (the first chunk, and
+    // hardly ever again): probabilities stay below 2^8, and the sums are not rescaled at every chunk.
+    mx = colgroup_max(mx);
+    if (__any(mx > st[j].m + kMaxSlackLog2)) {
+      const float m_new = fmaxf(st[j].m, mx);
+      const float alpha = fast_exp2(st[j].m - (m_new == kNegInf ? 0.f : m_new));
+      st[j].m = m_new;
+      st[j].l *= alpha;
+#pragma unroll
+      for (int t = 0; t < DV / 16; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st[j].o[t][i] *= alpha;
+    }
+    const float mref = st[j].m == kNegInf ? 0.f : st[j].m;
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -137,16 +148,19 @@ __device__ __forceinline__ void dense_values(DecState<T, DK, DV> (&st)[NT], vec8
       p[i] = whole || (key >= lo && key < n) ? x : 0.f;
       sum += p[i];
     }
-    st[j].l = st[j].l * alpha + sum;
-    st[j].m = m_new;
-    // probabilities are rounded to the tensors' type for the second product (at most half a step of each, the
-    // denominator keeps fp32); the sums stay in fp32
+    st[j].l += sum;
+    // The second product takes 16-bit probabilities: a rounded one and what the rounding left, each with its own matrix
+    // instructions (the loads are the bound), so that only the rounding of the result remains.
     const vec8_t<T> pb = pack8<T>(p);
+    vec8_t<T> rest = zero8<T>();
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) rest[i] = (T)(p[i] - (float)pb[i]);
+    }
 #pragma unroll
     for (int t = 0; t < DV / 16; ++t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) st[j].o[t][i] *= alpha;
       st[j].o[t] = mma16(v[t], pb, st[j].o[t]);
+      if constexpr (sizeof(T) == 2) st[j].o[t] = mma16(v[t], rest, st[j].o[t]);
     }
   }
 }

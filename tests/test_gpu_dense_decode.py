@@ -3,11 +3,13 @@ plain float64 softmax over the same cached tokens.
 
 Bound of the error, from the roundings the kernel makes (u = eps / 2 of the tensors' type, f = 2^-24 of fp32):
   scores    a sum of dk products in fp32, times the scale: |ds| <= (dk + 8) f |scale| sum |q k|
-  p         off by 2 ds (numerator and denominator) and by 2^-21 (the exponential), then rounded to the tensors' type: u
+  p         off by 2 ds (numerator and denominator) and by 2^-21 (the exponential); the second product takes it as a rounded
+            16-bit value and the rounded rest: off by u^2 of itself, or by 2^-25 where a float16 rest has no smaller step
   sums      a wavefront adds a quarter of the visible keys one after another at worst, then joins: (n / 4 + 64) f
   out       rounded once: u |out|
-With A = sum p |v| / l, |out - exact| <= u (|out| + A) + A (4 ds + 2^-20 + 2 (n / 4 + 64) f); the same terms without v for
-the log-sum-exp."""
+With A = sum p |v| / l and l >= 1 (the largest p is at least 1),
+|out - exact| <= u |out| + A (4 ds + 2^-20 + u^2 + 2 (n / 4 + 64) f) + [float16] 2^-25 n max |v|; the same terms without v and
+without the 16-bit ones for the log-sum-exp."""
 import math
 import random
 
@@ -60,7 +62,7 @@ def make_cache(paged, lens, cap, hkv, dk, dv, dtype, seed, garbage=None):
 def plain(q, k, v, scale, window):
     """q [Hq,Dk], k [n,Hkv,Dk], v [n,Hkv,Dv] -> float64 out [Hq,Dv], lse [Hq] and the error bounds of both."""
     hq, hkv, n = q.shape[0], k.shape[1], k.shape[0]
-    u = torch.finfo(q.dtype).eps / 2
+    u, half = torch.finfo(q.dtype).eps / 2, q.dtype == torch.float16
     lo = max(0, n - window) if window else 0
     q, k, v = q.double(), k.double()[lo:], v.double()[lo:]
     if n == 0:
@@ -76,7 +78,9 @@ def plain(q, k, v, scale, window):
     lse = torch.logsumexp(s, -1).reshape(hq)
     ds = ((q.shape[1] + 8) * F * abs(scale) * torch.matmul(qg.abs(), kt.abs()).amax(-1)).reshape(hq)
     chain = 2 * ((n - lo) / 4 + 64) * F
-    tol = u * (out.abs() + A) + A * (4 * ds[:, None] + 2.0 ** -20 + chain)
+    tol = u * out.abs() + A * (4 * ds[:, None] + 2.0 ** -20 + u * u + chain)
+    if half:
+        tol = tol + 2.0 ** -25 * (n - lo) * v.abs().max()
     tol_lse = 2 * ds + 2.0 ** -20 + chain + 4 * F * lse.abs()
     return out, lse, tol, tol_lse
 
