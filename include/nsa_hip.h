@@ -203,7 +203,8 @@ int nsa_qkv_rope(void* packed, void* q, void* k, void* v, void* gates, const flo
  * rotary channels turns by positions[pair_axis[i]][t] * inv_freq[i].
  *   positions int32 [axes][total], axes 1..4;  pair_axis int32 [rope_dim / 2], a HOST pointer, read during the call
  * The angle is formed in 64 bits, so that far positions keep their phase.  inv_freq is required; the other arguments are
- * those of nsa_qkv_rope.  pack = 1 also clears the columns of a row behind the last of the four ranges.  The reference's
+ * those of nsa_qkv_rope.  pack = 1 also clears the columns of a row behind the last of the four
+ * ranges, which must not overlap then.  The reference's
  * caller rotates before NSAAttention.forward (nsa/nsa.py:83-135); it has no kernel for it. */
 int nsa_qkv_rope_axes(void* packed, void* q, void* k, void* v, void* gates, const float* inv_freq,
                       const int32_t* positions, int axes, const int32_t* pair_axis, int64_t total, int ld, int q_off,
@@ -455,7 +456,7 @@ int nsa_decode_step_split_static(const void* q, const void* k_cache, const void*
 
 /* Dense decode attention: the one new token of every sequence attends ALL its cached tokens (window = 0) or the last
  * `window` of them, the current one among them.  Cache layouts as above; block_table NULL = contiguous caches (ctx_cap
- * used, a multiple of 64), else the paged pool of num_pages pages (max_pages used).  The compressed caches are not read.
+ * used, a multiple of 64, at most 2^30), else the paged pool of num_pages pages (max_pages used).  The compressed caches are not read.
  *   q [batch][hq][dk]   out [batch][hq][dv]   lse (optional) float [batch][hq]: natural-log log-sum-exp of the scaled scores
  * A sequence with ctx_lens[b] <= 0 yields out = 0 and lse = -inf; a length beyond the capacity counts as the capacity.
  * What the cache holds behind a sequence's last token, or before its window, does not matter (not even NaN).  A table
@@ -479,6 +480,7 @@ int nsa_dense_decode_step(const void* q, const void* k_cache, const void* v_cach
  * lengths[i] tokens of what slot parents[i] held before the call, for all i at once (slots[i] == parents[i] shortens a
  * sequence, length 0 empties it, length -1 is all the parent has).  Returns 0 with the bookkeeping updated and up to 2 n + 2 moves of 5 ints in `moves`;
  * NSA_ERR_INVALID or NSA_ERR_RESOURCE (not enough free pages) with nothing changed.
+ * nsa_paged_cache_grow (host) gives a slot pages from the free list until it holds `pages` of them, all or nothing.
  * nsa_paged_cache_move carries the moves out on the device (`moves` is a HOST pointer, read during the call): page table,
  * ctx_lens, last pages and compressed rows (block / stride as the cache was built), in one launch per 80 moves.
  * nsa_paged_cache_compact_plan (host) / nsa_paged_cache_compact_move (device; `pairs`, up to num_pages (page, new page)
@@ -486,6 +488,8 @@ int nsa_dense_decode_step(const void* q, const void* k_cache, const void* v_cach
 int nsa_paged_cache_plan(int32_t* table, int32_t* lens, int32_t* held, int32_t* refs, int32_t* free_pages, int32_t* n_free,
                          int batch, int max_pages, int num_pages, const int32_t* slots, const int32_t* parents,
                          const int32_t* lengths, int n, int32_t* moves, int32_t* n_moves);
+int nsa_paged_cache_grow(int32_t* table, int32_t* lens, int32_t* held, int32_t* refs, int32_t* free_pages, int32_t* n_free,
+                         int batch, int max_pages, int num_pages, int slot, int pages);
 int nsa_paged_cache_move(void* k_pool, void* v_pool_t, int32_t* block_table, void* ck_cache, void* cv_cache_t,
                          int32_t* ctx_lens, const int32_t* moves, int n_moves, int batch, int max_pages, int num_pages,
                          int hkv, int dk, int dv, int nc_cap, int block, int stride, int dtype, nsa_stream_t stream);

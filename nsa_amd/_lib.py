@@ -68,6 +68,7 @@ SIGNATURES = {
     "nsa_dense_decode_workspace_bytes": (_L, [_I] * 8),
     "nsa_dense_decode_step": (_I, [_P] * 4 + [_I, _I] + [_P] * 3 + [_I] * 7 + [_F, _I, _P, _L, _P]),
     "nsa_paged_cache_plan": (_I, [_P] * 6 + [_I] * 3 + [_P] * 3 + [_I] + [_P] * 2),
+    "nsa_paged_cache_grow": (_I, [_P] * 6 + [_I] * 5),
     "nsa_paged_cache_move": (_I, [_P] * 7 + [_I] * 11 + [_P]),
     "nsa_paged_cache_compact_plan": (_I, [_P] * 6 + [_I] * 3 + [_P] * 3),
     "nsa_paged_cache_compact_move": (_I, [_P] * 4 + [_I] * 8 + [_P]),

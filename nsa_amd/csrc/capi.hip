@@ -352,6 +352,11 @@ int nsa_qkv_rope_axes(void* packed, void* q, void* k, void* v, void* gates, cons
     return fail(NSA_ERR_INVALID, "qkv_rope_axes: pointers must be 16-byte aligned");
   a.base = nsa::QkvRopeArgs{packed, q, k, v, gates, inv_freq, positions, nullptr, 0, (long)total, ld, q_off, k_off, v_off,
                             g_off, hq, hkv, dk, dv, rope_off, rope_dim, interleaved ? 1 : 0, pack ? 1 : 0, dtype};
+  const int64_t at[4][2] = {{q_off, nq}, {k_off, nk}, {v_off, nv}, {g_off, gates ? ng : 0}};
+  for (int i = 0; i < 4 && pack; ++i)
+    for (int j = 0; j < i; ++j)
+      if (at[i][0] < at[j][0] + at[j][1] && at[j][0] < at[i][0] + at[i][1])
+        return fail(NSA_ERR_INVALID, "qkv_rope_axes: the column ranges of a packed row overlap");
   int64_t end = q_off + nq;
   if (k_off + nk > end) end = k_off + nk;
   if (v_off + nv > end) end = v_off + nv;
@@ -850,7 +855,7 @@ static bool finite_bits(float x) {
   return (u & 0x7f800000u) != 0x7f800000u;
 }
 static bool dense_sizes_ok(int batch, int hq, int hkv, int ctx_cap, int window) {
-  return batch > 0 && hq > 0 && hkv > 0 && hq % hkv == 0 && ctx_cap > 0 && ctx_cap % 64 == 0 && window >= 0 &&
+  return batch > 0 && hq > 0 && hkv > 0 && hq % hkv == 0 && ctx_cap > 0 && ctx_cap <= 1 << 30 && ctx_cap % 64 == 0 && window >= 0 &&
          (int64_t)batch * (ctx_cap / 64) <= 0x7fffffff;
 }
 
@@ -867,12 +872,12 @@ int nsa_dense_decode_step(const void* q, const void* k_cache, const void* v_cach
   if (!dtype_ok(dtype)) return fail(NSA_ERR_INVALID, "dense_decode: bad dtype");
   if (block_table) {
     if (max_pages <= 0 || num_pages <= 0) return fail(NSA_ERR_INVALID, "dense_decode: a block table needs max_pages and num_pages");
-    if (max_pages > 0x7fffffff / 64) return fail(NSA_ERR_INVALID, "dense_decode: max_pages too large");
+    if (max_pages > (1 << 30) / 64) return fail(NSA_ERR_INVALID, "dense_decode: more than 2^30 tokens per sequence");
     ctx_cap = max_pages * 64;
   }
   if (!dense_sizes_ok(batch, hq, hkv, ctx_cap, window))
-    return fail(NSA_ERR_INVALID, "dense_decode: sizes must be positive, hq a multiple of hkv, ctx_cap of 64, window >= 0 and "
-                                 "batch * pages below 2^31");
+    return fail(NSA_ERR_INVALID, "dense_decode: sizes must be positive, hq a multiple of hkv, ctx_cap of 64 and at most "
+                                 "2^30, window >= 0 and batch * pages below 2^31");
   if (!finite_bits(scale)) return fail(NSA_ERR_INVALID, "dense_decode: scale must be finite");
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache_t) || !aligned16(out))
     return fail(NSA_ERR_INVALID, "dense_decode: pointers must be 16-byte aligned");
@@ -906,12 +911,23 @@ int nsa_paged_cache_plan(int32_t* table, int32_t* lens, int32_t* held, int32_t* 
   try {
     const int rc = nsa::paged_plan(bk, slots, parents, lengths, n, moves, n_moves);
     if (rc == -1) return fail(NSA_ERR_INVALID, "paged_cache_plan: slots must be different slots of the cache, parents slots of the "
-                                               "cache, and no length beyond the parent's tokens");
+                                               "cache, no length beyond the parent's tokens, and every page of the pool");
     if (rc == -3) return fail(NSA_ERR_RESOURCE, "the K/V page pool is exhausted");
     return rc;
   } catch (...) {
     return fail(NSA_ERR_RESOURCE, "paged_cache_plan: out of host memory");
   }
+}
+
+int nsa_paged_cache_grow(int32_t* table, int32_t* lens, int32_t* held, int32_t* refs, int32_t* free_pages, int32_t* n_free,
+                         int batch, int max_pages, int num_pages, int slot, int pages) {
+  nsa::PagedBooks bk;
+  const int rc0 = paged_books("paged_cache_grow", &bk, table, lens, held, refs, free_pages, n_free, batch, max_pages, num_pages);
+  if (rc0 != NSA_OK) return rc0;
+  const int rc = nsa::paged_grow(bk, slot, pages);
+  if (rc == -1) return fail(NSA_ERR_INVALID, "paged_cache_grow: slot %d or %d pages outside the cache", slot, pages);
+  if (rc == -3) return fail(NSA_ERR_RESOURCE, "the K/V page pool is exhausted");
+  return rc;
 }
 
 int nsa_paged_cache_compact_plan(int32_t* table, int32_t* lens, int32_t* held, int32_t* refs, int32_t* free_pages,
@@ -922,7 +938,9 @@ int nsa_paged_cache_compact_plan(int32_t* table, int32_t* lens, int32_t* held, i
   if (rc != NSA_OK) return rc;
   if (!pairs || !n_pairs || !used) return fail(NSA_ERR_INVALID, "paged_cache_compact_plan: null pointer");
   try {
-    return nsa::paged_compact_plan(bk, pairs, n_pairs, used);
+    const int rc2 = nsa::paged_compact_plan(bk, pairs, n_pairs, used);
+    if (rc2 == -1) return fail(NSA_ERR_INVALID, "paged_cache_compact_plan: the table names a page outside the pool");
+    return rc2;
   } catch (...) {
     return fail(NSA_ERR_RESOURCE, "paged_cache_compact_plan: out of host memory");
   }

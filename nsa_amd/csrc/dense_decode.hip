@@ -189,7 +189,7 @@ dense_decode_kernel(const DenseDecodeArgs a) {
 
   // the plan: which sequence this unit belongs to, and which of its units it is
   int b = a.part == nullptr ? unit : -1, idx = 0, count = 1, before = 0;
-  const int C = a.part == nullptr ? a.ctx_cap : dense_unit_pages(a);
+  const int C = a.part == nullptr ? (a.ctx_cap + 63) / 64 : dense_unit_pages(a);
   for (int b0 = 0; b0 < a.batch && b < 0; b0 += 64) {
     const int mine = b0 + lane;
     const int nu = mine < a.batch ? dense_units_of(dense_span(a.ctx_lens[mine], a.ctx_cap, a.window).pages, C) : 0;

@@ -166,6 +166,7 @@ constexpr int kPagedCyclePiece = 64;   // moves of a cycle that stay together
 constexpr int kPagedPairs = 384;       // pages per launch of a compaction
 int paged_plan(const PagedBooks& bk, const int32_t* slots, const int32_t* parents, const int32_t* lengths, int n,
                int32_t* moves, int32_t* n_moves);
+int paged_grow(const PagedBooks& bk, int slot, int pages);
 int paged_compact_plan(const PagedBooks& bk, int32_t* pairs, int32_t* n_pairs, int32_t* used);
 struct PagedPools { void* k_pool; void* v_pool; long k_page, v_page; };   // 16-byte vectors per page
 struct PagedMove { int src, dst, len, rows, tail, round; };               // round: moves of the round that starts here

@@ -170,6 +170,33 @@ paged_compact_kernel(const PagedCompactArgs a) {
 
 // ------------------------------------------------------------------------------------------------ host half
 
+// Whether slot b's pages are pages of the pool, and enough for its tokens.
+static bool slot_ok(const PagedBooks& bk, int b) {
+  if (bk.held[b] < 0 || bk.held[b] > bk.max_pages || bk.lens[b] < 0 || bk.lens[b] > bk.held[b] * 64L) return false;
+  const int32_t* t = bk.table + (long)b * bk.max_pages;
+  bool bad = false;
+  for (int k = 0; k < bk.held[b]; ++k) bad |= (unsigned)(t[k] - 1) >= (unsigned)(bk.num_pages - 1);
+  return !bad;
+}
+
+// Slot `slot` comes to hold `pages` pages if it holds fewer; the new ones are the top of the free list.
+int paged_grow(const PagedBooks& bk, int slot, int pages) {
+  if (slot < 0 || slot >= bk.batch || pages < 0 || pages > bk.max_pages || !slot_ok(bk, slot)) return -1;
+  const int more = pages - bk.held[slot];
+  if (more <= 0) return 0;
+  if (more > *bk.n_free) return -3;
+  if (*bk.n_free > bk.num_pages) return -1;
+  for (int k = 0; k < more; ++k)
+    if ((unsigned)(bk.free_pages[*bk.n_free - 1 - k] - 1) >= (unsigned)(bk.num_pages - 1)) return -1;
+  int32_t* t = bk.table + (long)slot * bk.max_pages + bk.held[slot];
+  for (int k = 0; k < more; ++k) {
+    t[k] = bk.free_pages[--*bk.n_free];
+    bk.refs[t[k]] = 1;
+  }
+  bk.held[slot] = pages;
+  return 0;
+}
+
 // Moves 0..n-1 (5 ints each: src, dst, len, last page read, last page written) in an order that is right one after the
 // other; src -1 / dst -1 is the register that holds a cycle's first slot.  A length of -1 is all the parent has.  Returns 0,
 // -1 (bad argument) or -3 (pool exhausted); nothing changes unless it returns 0.
@@ -181,9 +208,11 @@ int paged_plan(const PagedBooks& bk, const int32_t* slots, const int32_t* parent
   std::vector<int> ready;
   std::vector<int32_t> old;
   ready.reserve(n);                                      // nothing below the first change allocates
+  if (*bk.n_free < 0 || *bk.n_free > bk.num_pages) return -1;
   for (int i = 0; i < n; ++i) {
     const int s = slots[i], p = parents[i];
-    if (s < 0 || s >= B || p < 0 || p >= B || node[s] >= 0) return -1;
+    if (s < 0 || s >= B || p < 0 || p >= B || node[s] >= 0 || !slot_ok(bk, s)) return -1;
+    if (row_of[p] < 0 && !slot_ok(bk, p)) return -1;
     lengths[i] = asked[i] == -1 ? bk.lens[p] : asked[i];
     if (lengths[i] < 0 || lengths[i] > bk.lens[p]) return -1;
     node[s] = i;
@@ -242,17 +271,20 @@ int paged_plan(const PagedBooks& bk, const int32_t* slots, const int32_t* parent
     for (int k = bk.held[slots[i]] - 1; k >= common[i]; --k) {
       const int pg = own(i)[k];
       if (bk.refs[pg] == 0) {
+        if (nf >= bk.num_pages) continue;                // cannot be while the books are in order
         bk.refs[pg] = -1;
         bk.free_pages[nf++] = pg;
       }
     }
   for (int k = free0; k < nf; ++k) bk.refs[bk.free_pages[k]] = 0;
-  if (missing > nf) {
+  bool bad = false;                                      // a free list that names pages outside the pool
+  for (int k = 0; k < std::min(missing, nf); ++k) bad |= (unsigned)(bk.free_pages[nf - 1 - k] - 1) >= (unsigned)(bk.num_pages - 1);
+  if (missing > nf || bad) {
     for (int i = 0; i < n; ++i)
       if (tail[i] >= 0) bk.refs[tail[i]] = 0;
     share(-1);
     drop(-1);
-    return -3;
+    return bad ? -1 : -3;
   }
   for (int i = 0; i < n; ++i)
     if (from[i] >= 0 && tail[i] < 0) {
@@ -319,6 +351,8 @@ int paged_plan(const PagedBooks& bk, const int32_t* slots, const int32_t* parent
 
 // Pairs (page, new page) after which the pages in use are 1..used.
 int paged_compact_plan(const PagedBooks& bk, int32_t* pairs, int32_t* n_pairs, int32_t* used) {
+  for (int b = 0; b < bk.batch; ++b)
+    if (!slot_ok(bk, b)) return -1;
   int live = 0;
   for (int p = 1; p < bk.num_pages; ++p) live += bk.refs[p] > 0;
   std::vector<int32_t> to(bk.num_pages, 0);

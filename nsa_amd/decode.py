@@ -97,15 +97,6 @@ class _FreePages:
     def __setitem__(self, i, page):
         self.ids[self._at(i)] = page
 
-    def pop(self):
-        page = self[-1]
-        self.n.value -= 1
-        return page
-
-    def append(self, page):
-        self.ids[self.n.value] = page
-        self.n.value += 1
-
 
 class NSAPagedDecodeCache:
     """The same caches with K and V in a pool of 64-token pages shared by all sequences (one page =
@@ -156,6 +147,21 @@ class NSAPagedDecodeCache:
     def free_pages(self) -> int:
         return len(self._free)
 
+    def _books(self):
+        return (self._table, self._lens, self._held, self._refs, self._free.ids, C.byref(self._free.n), self.batch,
+                self.max_pages, self.num_pages)
+
+    def _plan(self, slots, parents, lengths):
+        """Host half of a fork or move: the bookkeeping, all or nothing; returns the moves for the device."""
+        n = len(slots)
+        ints = C.c_int32 * n
+        moves, n_moves = (C.c_int32 * (10 * n + 10))(), C.c_int32()
+        rc = _lib.load().nsa_paged_cache_plan(*self._books(), ints(*slots), ints(*parents), ints(*lengths), n, moves,
+                                              C.byref(n_moves))
+        if rc:
+            _lib.check(rc, "nsa_paged_cache_plan")
+        return moves, n_moves.value
+
     def _pages_of(self, b: int):
         at = b * self.max_pages
         return self._table[at:at + self._held[b]]
@@ -168,18 +174,15 @@ class NSAPagedDecodeCache:
         """Makes sure sequence b owns pages for new_len tokens; returns the (slot, page) pairs added.
         All or nothing: on an error the sequence keeps exactly the pages it had."""
         need, held = (new_len + self.PAGE - 1) // self.PAGE, self._held[b]
+        if need <= held:
+            return []
         if need > self.max_pages:
             raise RuntimeError(f"sequence {b} would exceed the cache capacity of {self.ctx_cap} tokens")
         if need - held > len(self._free):
             raise RuntimeError("the K/V page pool is exhausted")
-        added = []
-        for slot in range(held, need):
-            pg = self._free.pop()
-            added.append((slot, pg))
-            self._table[b * self.max_pages + slot] = pg
-            self._refs[pg] = 1
-        self._held[b] = max(held, need)
-        return added
+        _lib.check(_lib.load().nsa_paged_cache_grow(*self._books(), b, need), "nsa_paged_cache_grow")
+        at = b * self.max_pages
+        return list(enumerate(self._table[at + held:at + need], held))
 
     def _publish(self, entries):
         """entries: (sequence, slot, page) triples to write into the device block table."""
@@ -191,15 +194,8 @@ class NSAPagedDecodeCache:
 
     def release(self, b: int):
         """Empties sequence b; the pages that no other sequence shares go back to the pool."""
-        at = b * self.max_pages
-        for slot in range(self._held[b] - 1, -1, -1):
-            pg = self._table[at + slot]
-            self._refs[pg] -= 1
-            if self._refs[pg] == 0:
-                self._free.append(pg)
-            self._table[at + slot] = 0
-        self._held[b] = 0
-        self._lens[b] = 0
+        b = range(self.batch)[b]
+        self._plan([b], [b], [0])
         self.block_table[b].zero_()
         self.ctx_lens[b] = 0
 
@@ -209,7 +205,7 @@ class NSAPagedDecodeCache:
         B == batch), or k [T,Hkv,Dk], v [T,Hkv,Dv] for sequence `seq` alone."""
         from . import ops
         if seq is not None:
-            k, v, seqs = k.unsqueeze(0), v.unsqueeze(0), [seq]
+            k, v, seqs = k.unsqueeze(0), v.unsqueeze(0), [range(self.batch)[seq]]
         else:
             seqs = list(range(self.batch))
         B, T = k.shape[:2]
@@ -225,6 +221,8 @@ class NSAPagedDecodeCache:
             held = sum(self._held[b] for b in seqs)
         if len(seqs) * ((T + self.PAGE - 1) // self.PAGE) > len(self._free) + held:
             raise RuntimeError("the K/V page pool is exhausted")       # before any sequence is touched
+        if T > self.ctx_cap:
+            raise RuntimeError(f"sequence {seqs[0]} would exceed the cache capacity of {self.ctx_cap} tokens")
         entries = []
         if self._shares:
             for b in seqs:
@@ -272,17 +270,12 @@ class NSAPagedDecodeCache:
                 return self._assign(slots, parents, lengths)
         if self.dk % 8 or self.dv % 8:
             raise NotImplementedError("forks and moves take head dims that are multiples of 8")
-        lib, ints, code = _lib.load(), C.c_int32 * n, _dtype_code(self.k_pool)
-        moves, n_moves = (C.c_int32 * (10 * n + 10))(), C.c_int32()
-        rc = lib.nsa_paged_cache_plan(self._table, self._lens, self._held, self._refs, self._free.ids, C.byref(self._free.n),
-                                      self.batch, self.max_pages, self.num_pages, ints(*slots), ints(*parents),
-                                      ints(*lengths), n, moves, C.byref(n_moves))
-        if rc:
-            _lib.check(rc, "nsa_paged_cache_plan")
+        code = _dtype_code(self.k_pool)
+        moves, n_moves = self._plan(slots, parents, lengths)
         self._shares = True
-        rc = lib.nsa_paged_cache_move(
+        rc = _lib.load().nsa_paged_cache_move(
             self.k_pool.data_ptr(), self.v_pool_t.data_ptr(), self.block_table.data_ptr(), self.ck.data_ptr(),
-            self.cvt.data_ptr(), self.ctx_lens.data_ptr(), moves, n_moves.value, self.batch, self.max_pages, self.num_pages,
+            self.cvt.data_ptr(), self.ctx_lens.data_ptr(), moves, n_moves, self.batch, self.max_pages, self.num_pages,
             self.hkv, self.dk, self.dv, self.nc_cap, self.block, self.stride, code, _raw_stream(device))
         if rc:
             _lib.check(rc, "nsa_paged_cache_move")
@@ -337,9 +330,7 @@ class NSAPagedDecodeCache:
             raise NotImplementedError("forks and moves take head dims that are multiples of 8")
         lib, code = _lib.load(), _dtype_code(self.k_pool)
         pairs, n_pairs, used = (C.c_int32 * (2 * self.num_pages))(), C.c_int32(), C.c_int32()
-        rc = lib.nsa_paged_cache_compact_plan(self._table, self._lens, self._held, self._refs, self._free.ids,
-                                              C.byref(self._free.n), self.batch, self.max_pages, self.num_pages, pairs,
-                                              C.byref(n_pairs), C.byref(used))
+        rc = lib.nsa_paged_cache_compact_plan(*self._books(), pairs, C.byref(n_pairs), C.byref(used))
         _lib.check(rc, "nsa_paged_cache_compact_plan")
         rc = lib.nsa_paged_cache_compact_move(
             self.k_pool.data_ptr(), self.v_pool_t.data_ptr(), self.block_table.data_ptr(), pairs, n_pairs.value, self.batch,
@@ -350,15 +341,16 @@ class NSAPagedDecodeCache:
     def reserve_next(self):
         """Host half of append(): makes sure every sequence owns the page of its next token and
         publishes new table entries.  Separate so that the device half can live in a captured graph."""
-        fresh = sum(self._lens[b] % self.PAGE == 0 for b in range(self.batch))
-        if fresh > len(self._free):
+        lens = self._lens[:]
+        fresh = [b for b, n in enumerate(lens) if n % self.PAGE == 0]
+        if len(fresh) > len(self._free):
             raise RuntimeError("the K/V page pool is exhausted")       # before any sequence has grown
-        if max(self._lens) >= self.ctx_cap:
+        if max(lens) >= self.ctx_cap:
             raise RuntimeError(f"a sequence would exceed the cache capacity of {self.ctx_cap} tokens")
         entries = []
-        for b in range(self.batch):
-            entries += [(b, slot, pg) for slot, pg in self._grow(b, self._lens[b] + 1)]
-            self._lens[b] += 1
+        for b in fresh:
+            entries += [(b, slot, pg) for slot, pg in self._grow(b, lens[b] + 1)]
+        self._lens[:] = [n + 1 for n in lens]
         self._publish(entries)
 
     @torch.no_grad()
@@ -541,12 +533,14 @@ def dense_decode_step(q: torch.Tensor, cache, scale: Optional[float] = None, sli
     elif out.shape != (B, hq, dv) or out.dtype != q.dtype or out.device != device or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise ValueError("out must be a contiguous, 16-byte aligned [B,Hq,Dv] tensor of q's dtype and device")
+    if out.data_ptr() == q.data_ptr():
+        raise ValueError("out must not be q: workgroups still read the query when others write")
     if lse is None:
         if return_lse:
             lse = torch.empty((B, hq), dtype=torch.float32, device=device)
     elif lse.shape != (B, hq) or lse.dtype != torch.float32 or lse.device != device or not lse.is_contiguous():
         raise ValueError("lse must be a contiguous float32 [B,Hq] tensor on q's device")
-    code = _dtype_code(q)
+    code, sliding_window = _dtype_code(q), min(sliding_window, cache.ctx_cap)
     need = _dense_workspace_bytes(B, hq, hkv, dk, dv, cache.ctx_cap, sliding_window, code)
     # a workspace of this call's own: two captured graphs, or two streams, never share one
     ws = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None

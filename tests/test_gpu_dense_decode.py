@@ -264,6 +264,24 @@ def test_buffers_strides_and_streams():
         b = dense_decode_step(q, c)
     torch.cuda.current_stream().wait_stream(side)
     assert a is out and torch.equal(out, want) and torch.equal(lse, want_lse) and torch.equal(b, want)
+    assert torch.equal(dense_decode_step(q, c, sliding_window=2 ** 40), want)
+
+
+def test_refusals():
+    from nsa_amd.decode import dense_decode_step
+    c, _, _ = make_cache(True, [500, 3], 512, 2, 64, 64, torch.bfloat16, seed=115)
+    q = torch.zeros(2, 8, 64, dtype=torch.bfloat16, device=DEV)
+    z = dict(dtype=torch.bfloat16, device=DEV)
+    for bad in (dict(q=q[:1]), dict(q=q[0]), dict(q=q[..., :32]), dict(q=q.half()), dict(q=q[:, :7]), dict(q=q[:, :0]),
+                dict(out=torch.empty(2, 8, 32, **z)), dict(out=torch.empty(2, 8, 64, device=DEV)), dict(out=q),
+                dict(out=torch.empty(8, 2, 64, **z).transpose(0, 1)), dict(out=torch.empty(2 * 8 * 64 + 4, **z)[4:].view(2, 8, 64)),
+                dict(lse=torch.empty(2, 8, **z)), dict(lse=torch.empty(2, 4, device=DEV)), dict(sliding_window=-1),
+                dict(scale=float("nan")), dict(scale=float("inf"))):
+        with pytest.raises(ValueError):
+            dense_decode_step(**dict(dict(q=q, cache=c), **bad))
+    wide, _, _ = make_cache(True, [5], 64, 1, 96, 96, torch.bfloat16, seed=116)
+    with pytest.raises(NotImplementedError):
+        dense_decode_step(torch.zeros(1, 2, 96, **z), wide)
 
 
 def test_captured_calls_follow_the_growing_cache():

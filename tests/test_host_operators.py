@@ -70,6 +70,7 @@ def test_rope_axes_argument_errors_do_not_launch(lib):
                 dict(axes=2), dict(pair_axis=pairs(-1)), dict(packed=p + 4), dict(hq=1 << 26)):
         assert call(**bad) == -1, bad
         assert lib.nsa_last_error_string()
+    assert call(pack=1, k_off=248) == -1 and call(pack=1, g_off=380) == -1              # ranges of a packed row overlap
     assert call(dk=512, rope_dim=512, ld=8192, k_off=2048, v_off=4096, g_off=6000) == -2
 
 
@@ -412,6 +413,53 @@ def test_paged_cache_python_checks():
     assert c._lens[0] == 10 and c.free_pages == 5
     with pytest.raises(IndexError):
         c._free[5]
-    c.release(0)
-    with pytest.raises(IndexError):
-        [c._free.pop() for _ in range(7)]
+    c.release(-3)                                                                # slots count from the end, as lists do
+    assert c.free_pages == 6 and c._lens[0] == 0 and list(c._refs) == [0] * 7
+    for b in (3, -4):
+        with pytest.raises(IndexError):
+            c.release(b)
+
+
+def test_paged_books_that_are_not_in_order_are_refused(lib):
+    """page ids outside the pool, in the table or in the free list, and counts that cannot be: refused, nothing changed"""
+    for spoil in range(6):
+        c = small_cache(3, 6)
+        m = Model(c)
+        m.append(0, 100)
+        if spoil == 0:
+            c._table[1] = 7
+        elif spoil == 1:
+            c._table[0] = 0
+        elif spoil == 2:
+            c._held[0] = 6
+        elif spoil == 3:
+            c._lens[0] = 129
+        elif spoil == 4:
+            c._free.n.value = 9
+        else:
+            c._free[-1] = 7
+        before = books(c) if spoil != 4 else list(c._refs)
+        assert plan(lib, c, [1, 2], [0, 0], [70, 70])[0] == -1
+        if spoil != 5:
+            assert plan(lib, c, [0], [0], [0])[0] == -1
+        if spoil not in (4, 5):
+            n = (ctypes.c_int32 * 20)()
+            assert lib.nsa_paged_cache_compact_plan(*c._books(), n, ctypes.byref(ctypes.c_int32()),
+                                                    ctypes.byref(ctypes.c_int32())) == -1
+        assert lib.nsa_paged_cache_grow(*c._books(), 0 if spoil < 4 else 1, 3) == -1
+        assert before == (books(c) if spoil != 4 else list(c._refs))
+    c = small_cache(2, 6)
+    for slot, pages, rc in ((2, 1, -1), (-1, 1, -1), (0, 6, -1), (0, -1, -1), (0, 5, 0), (1, 2, -3), (0, 3, 0)):
+        assert lib.nsa_paged_cache_grow(*c._books(), slot, pages) == rc
+    assert c._held[0] == 5 and c._held[1] == 0 and c.free_pages == 1
+
+
+def test_a_copy_of_a_cache_has_books_of_its_own():
+    import copy
+    c = small_cache(2, 6)
+    Model(c).append(0, 70)
+    d = copy.deepcopy(c)
+    d.release(0)
+    assert d.free_pages == 6 and c.free_pages == 4 and c._lens[0] == 70
+    Model(d).append(1, 30)
+    assert c._held[1] == 0 and d._held[1] == 1
