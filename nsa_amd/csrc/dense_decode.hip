@@ -344,7 +344,8 @@ dense_decode_join_kernel(const DenseDecodeArgs a, int rows_per_slot, int blocks)
   for (int x = lane; x < b; x += 64) u0 += dense_units_of(dense_span(a.ctx_lens[x], a.ctx_cap, a.window).pages, C);
   u0 = wave_sum(u0);
   const int count = dense_units_of(dense_span(a.ctx_lens[b], a.ctx_cap, a.window).pages, C);
-  if (count <= 1) return;
+  // more units than there is room for: only if another stream changed the lengths between the two kernels
+  if (count <= 1 || u0 + count > a.units + a.batch) return;
   const int G = a.hq / a.hkv, h = head / G, r = head % G;
   const int per = a.hkv * blocks, hb = h * blocks + r / rows_per_slot;
   const long step = (long)per * rows_per_slot;
@@ -423,7 +424,11 @@ DensePlan dense_decode_plan(const DenseDecodeArgs& a) {
   // workgroups, 767 with 512, 791 with 768; 16 of them at 64 / 64: 108, 102, 105 us)
   const long in_flight = 32L * kDenseWaves * (a.dk + a.dv) * (a.dtype == 1 ? 4 : 2);
   const long workgroups = 256 * min(4L, max(1L, 65536 / in_flight));
-  p.units = (int)max(1L, min(workgroups / per, (long)a.batch * span));
+  // With more sequences than that they come in several rounds anyway; a third of a sequence per unit keeps the last round
+  // short (32 / 4 heads of 128 bf16, one unit per sequence against three: 65 sequences of 8192 323 and 247 us, 100 of up
+  // to 8192 252 and 190, 200 of up to 4096 225 and 201; 128 of 4096, which are two rounds to the dot, 200 and 220).
+  const long aim = a.batch > workgroups / per ? 3L * a.batch : workgroups / per;
+  p.units = (int)max(1L, min(aim, (long)a.batch * span));
   // A short capacity is not worth a second launch: 8 wavefronts take the whole sequence.  16 / 4 heads, split against
   // whole, us: one sequence of 512 tokens, 64 / 64 bf16 9.0, 6.7, of 1024 8.8, 10.3; 128 / 128 bf16
   // 256 tokens 9.7, 6.7, 512 9.7, 10.3; 64 / 64 fp32 256 tokens 10.1, 6.9, 512 10.1, 11.8.  64 sequences fill the card
