@@ -9,7 +9,7 @@
 // so even the moves of a permutation need no second buffer: what it has not read yet, nobody has written.  A cycle keeps
 // its first slot's 16 bytes in a register.  Loads of up to 8 moves travel together, and moves that read the same slot
 // share one load.  Bound by HBM: every source is read once, every copy written once (32749 tokens, 4 heads of 128 / 128
-// bf16, into 63 slots: 56 us, 4.9 TB/s; half of 64 slots of 16411 tokens onto the other half: 26 us, 5.5 TB/s), and by the
+// bf16, into 63 slots: 53 us, 5.2 TB/s; half of 64 slots of 16411 tokens onto the other half: 26 us, 5.5 TB/s), and by the
 // latency of the walk where the slots hold little (a cycle of 16 slots of 4096 tokens: 8.8 us).
 #include <algorithm>
 #include <vector>
@@ -386,15 +386,18 @@ int paged_compact_plan(const PagedBooks& bk, int32_t* pairs, int32_t* n_pairs, i
 
 static long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
-// Moves that do not depend on one another may run side by side: where the slots hold little, one thread walking over all of
-// them would be slow (300 tokens forked into 63 slots: 31 us, side by side 7).  Puts the moves of a launch into groups of
-// about `want` moves, in which what depends on one another stays together and in order.
-static void paged_groups(PagedMoveArgs& a, const PagedMove* in, int n, int want) {
+// Puts the moves of a launch into groups of about kPagedGroup, in which what depends on one another stays together and in
+// order; groups run side by side.  4: one walk over all moves is slow where the slots hold little (300 tokens forked into 63
+// slots: 31 us, in groups of 32, 8, 4 and 1 13.4, 6.9, 7.0 and 11.4), and a source is read once per group (32749 tokens
+// into 63 slots: groups of 32, 8, 4 and 1 58, 54, 53 and 85 us).
+constexpr int kPagedGroup = 4;
+
+static void paged_groups(PagedMoveArgs& a, const PagedMove* in, int n) {
   int root[kPagedMoves], order[kPagedMoves];
   for (int i = 0; i < n; ++i) root[i] = i;
   auto find = [&](int i) { while (root[i] != i) i = root[i]; return i; };
   auto join = [&](int i, int j) { i = find(i); j = find(j); root[std::max(i, j)] = std::min(i, j); };
-  if (want >= n) {
+  if (n <= kPagedGroup) {
     for (int i = 1; i < n; ++i) root[i] = 0;
   } else {
     int slot[256], writer[256];                          // a hash from a slot to the first move that writes it
@@ -426,7 +429,7 @@ static void paged_groups(PagedMoveArgs& a, const PagedMove* in, int n, int want)
     if (find(r) != r) continue;
     for (int i = r; i < n; ++i)
       if (find(i) == r) order[at++] = i;
-    if (at - a.group[groups] >= want) a.group[++groups] = at;
+    if (at - a.group[groups] >= kPagedGroup) a.group[++groups] = at;
   }
   if (a.group[groups] != at) a.group[++groups] = at;
   for (int i = 0; i < n; ++i) a.moves[i] = in[order[i]];
@@ -468,8 +471,7 @@ int launch_paged_move(PagedMoveArgs a, const int32_t* moves, int n, int block, i
     a.cv_blocks = ceil_div((long)a.hkv * a.dv * ceil_div(a.rows_most, vec), 256);
     a.table_blocks = ceil_div(a.max_pages, 256);
     const long slot_blocks = a.ck_blocks + a.cv_blocks + a.table_blocks;
-    // one walk over all moves where its workgroups fill the card (a source is then read once for all its copies)
-    paged_groups(a, list, end - i, (int)std::min<long>(kPagedMoves, std::max<long>(kPagedRound, (end - i) * slot_blocks / 1024)));
+    paged_groups(a, list, end - i);
     const long blocks = slot_blocks + pairs * per;
     if (blocks > 0x7fffffffL) return -2;
     const dim3 grid((unsigned)blocks, (unsigned)a.groups);
