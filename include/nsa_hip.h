@@ -478,7 +478,7 @@ int nsa_dense_decode_step(const void* q, const void* k_cache, const void* v_cach
  * [batch][max_pages] (0 = none), lens [batch] (tokens), held [batch] (pages), refs [num_pages] (slots that hold a page),
  * free_pages [num_pages] with *n_free entries (a stack; page 0 is never handed out).  Slot slots[i] becomes the first
  * lengths[i] tokens of what slot parents[i] held before the call, for all i at once (slots[i] == parents[i] shortens a
- * sequence, length 0 empties it, length -1 is all the parent has).  Returns 0 with the bookkeeping updated and up to 2 n + 2 moves of 5 ints in `moves`;
+ * sequence, length 0 empties it, length -1 is all the parent has, and so are lengths NULL).  Returns 0 with the bookkeeping updated and up to 2 n + 2 moves of 5 ints in `moves`;
  * NSA_ERR_INVALID or NSA_ERR_RESOURCE (not enough free pages) with nothing changed.
  * nsa_paged_cache_grow (host) gives a slot pages from the free list until it holds `pages` of them, all or nothing.
  * nsa_paged_cache_move carries the moves out on the device (`moves` is a HOST pointer, read during the call): page table,

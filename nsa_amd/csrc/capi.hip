@@ -906,7 +906,7 @@ int nsa_paged_cache_plan(int32_t* table, int32_t* lens, int32_t* held, int32_t* 
   nsa::PagedBooks bk;
   const int rc0 = paged_books("paged_cache_plan", &bk, table, lens, held, refs, free_pages, n_free, batch, max_pages, num_pages);
   if (rc0 != NSA_OK) return rc0;
-  if (n < 0 || (n > 0 && (!slots || !parents || !lengths || !moves)) || !n_moves)
+  if (n < 0 || (n > 0 && (!slots || !parents || !moves)) || !n_moves)
     return fail(NSA_ERR_INVALID, "paged_cache_plan: null pointer");
   try {
     const int rc = nsa::paged_plan(bk, slots, parents, lengths, n, moves, n_moves);

@@ -198,7 +198,7 @@ int paged_grow(const PagedBooks& bk, int slot, int pages) {
 }
 
 // Moves 0..n-1 (5 ints each: src, dst, len, last page read, last page written) in an order that is right one after the
-// other; src -1 / dst -1 is the register that holds a cycle's first slot.  A length of -1 is all the parent has.  Returns 0,
+// other; src -1 / dst -1 is the register that holds a cycle's first slot.  A length of -1 (no lengths: each) is all the parent has.  Returns 0,
 // -1 (bad argument) or -3 (pool exhausted); nothing changes unless it returns 0.
 int paged_plan(const PagedBooks& bk, const int32_t* slots, const int32_t* parents, const int32_t* asked, int n,
                int32_t* moves, int32_t* n_moves) {
@@ -213,7 +213,7 @@ int paged_plan(const PagedBooks& bk, const int32_t* slots, const int32_t* parent
     const int s = slots[i], p = parents[i];
     if (s < 0 || s >= B || p < 0 || p >= B || node[s] >= 0 || !slot_ok(bk, s)) return -1;
     if (row_of[p] < 0 && !slot_ok(bk, p)) return -1;
-    lengths[i] = asked[i] == -1 ? bk.lens[p] : asked[i];
+    lengths[i] = asked == nullptr || asked[i] == -1 ? bk.lens[p] : asked[i];
     if (lengths[i] < 0 || lengths[i] > bk.lens[p]) return -1;
     node[s] = i;
     if (row_of[p] < 0) {

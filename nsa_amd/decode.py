@@ -152,12 +152,13 @@ class NSAPagedDecodeCache:
                 self.max_pages, self.num_pages)
 
     def _plan(self, slots, parents, lengths):
-        """Host half of a fork or move: the bookkeeping, all or nothing; returns the moves for the device."""
+        """Host half of a fork or move: the bookkeeping, all or nothing; returns the moves for the device.  lengths None:
+        every slot gets all its parent has."""
         n = len(slots)
         ints = C.c_int32 * n
         moves, n_moves = (C.c_int32 * (10 * n + 10))(), C.c_int32()
-        rc = _lib.load().nsa_paged_cache_plan(*self._books(), ints(*slots), ints(*parents), ints(*lengths), n, moves,
-                                              C.byref(n_moves))
+        rc = _lib.load().nsa_paged_cache_plan(*self._books(), ints(*slots), ints(*parents),
+                                              None if lengths is None else ints(*lengths), n, moves, C.byref(n_moves))
         if rc:
             _lib.check(rc, "nsa_paged_cache_plan")
         return moves, n_moves.value
@@ -256,7 +257,8 @@ class NSAPagedDecodeCache:
 
     # -------------------------------------------------------------------------------- forks and moves of sequences
     def _assign(self, slots, parents, lengths):
-        """Slot slots[i] becomes the first lengths[i] tokens of what slot parents[i] held, for all i at once."""
+        """Slot slots[i] becomes the first lengths[i] tokens (lengths None: all) of what slot parents[i] held, for all i at
+        once."""
         n = len(slots)
         if n == 0:
             return
@@ -305,7 +307,7 @@ class NSAPagedDecodeCache:
             raise ValueError("reorder() got %d parents for %d slots" % (len(parents), self.batch))
         self._check_slot(min(parents))
         self._check_slot(max(parents))
-        self._assign(range(self.batch), parents, [-1] * self.batch)
+        self._assign(range(self.batch), parents, None)
 
     def truncate(self, seq: int, length: int):
         """Sequence seq keeps its first `length` tokens (a draft that was rejected); the pages behind them go back to the
