@@ -267,6 +267,25 @@ def test_buffers_strides_and_streams():
     assert torch.equal(dense_decode_step(q, c, sliding_window=2 ** 40), want)
 
 
+def test_calls_on_two_streams_at_once_share_nothing():
+    from nsa_amd.decode import dense_decode_step
+    lens = [3000, 700, 4000, 1]
+    c, ks, vs = make_cache(True, lens, 4032, 4, 128, 128, torch.bfloat16, seed=130)
+    qs = [randn(4, 64, 128, seed=131 + i, dtype=torch.bfloat16).to(DEV) for i in range(2)]
+    want = [check(q, c, ks, vs)[0] for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(dense_decode_step(qs[i], c))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in got[i])
+
+
 def test_refusals():
     from nsa_amd.decode import dense_decode_step
     c, _, _ = make_cache(True, [500, 3], 512, 2, 64, 64, torch.bfloat16, seed=115)
