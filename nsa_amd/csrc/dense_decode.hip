@@ -289,7 +289,7 @@ dense_decode_kernel(const DenseDecodeArgs a) {
     float M = kNegInf;
 #pragma unroll
     for (int x = 0; x < W; ++x) M = fmaxf(M, ml[x][n16][0]);
-    const float own = M == kNegInf ? 0.f : fast_exp2(st[j].m - M);
+    const float own = fast_exp2(st[j].m - (M == kNegInf ? 0.f : M));
 #pragma unroll
     for (int t = 0; t < DV / 16; ++t) {
       f32x4_t o = st[j].o[t];
@@ -307,7 +307,7 @@ dense_decode_kernel(const DenseDecodeArgs a) {
       f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int x = 0; x < W; ++x) {
-        if (Mr != kNegInf) L += ml[x][r][1] * fast_exp2(ml[x][r][0] - Mr);
+        L += ml[x][r][1] * fast_exp2(ml[x][r][0] - (Mr == kNegInf ? 0.f : Mr));
         o += *reinterpret_cast<const f32x4_t*>(&plane[x][r][d]);
       }
       if (count > 1) {
@@ -319,12 +319,12 @@ dense_decode_kernel(const DenseDecodeArgs a) {
           pm[1] = L;
         }
       } else {
-        const float inv = L > 0.f ? 1.0f / L : 0.f;
+        const float inv = L == 0.f ? 0.f : 1.0f / L;     // not L > 0: a NaN among the scores has to come through
         const long row = (long)b * a.hq + h * G + row0 + 16 * j + r;
         T* dst = reinterpret_cast<T*>(a.out) + row * DV + d;
 #pragma unroll
         for (int i = 0; i < 4; ++i) dst[i] = (T)(o[i] * inv);
-        if (a.lse != nullptr && d == 0) a.lse[row] = L > 0.f ? (Mr + __log2f(L)) * (1.0f / kLog2e) : kNegInf;
+        if (a.lse != nullptr && d == 0) a.lse[row] = L == 0.f ? kNegInf : (Mr + __log2f(L)) * (1.0f / kLog2e);
       }
     }
   }
@@ -399,8 +399,8 @@ dense_decode_join_kernel(const DenseDecodeArgs a, int rows_per_slot, int blocks)
     L = fmaf(red[k][1], wgt, L);
   }
   const long row = (long)b * a.hq + head;
-  reinterpret_cast<T*>(a.out)[row * DV + threadIdx.x] = (T)(L > 0.f ? sum / L : 0.f);
-  if (a.lse != nullptr && threadIdx.x == 0) a.lse[row] = L > 0.f ? (M + __log2f(L)) * (1.0f / kLog2e) : kNegInf;
+  reinterpret_cast<T*>(a.out)[row * DV + threadIdx.x] = (T)(L == 0.f ? 0.f : sum / L);
+  if (a.lse != nullptr && threadIdx.x == 0) a.lse[row] = L == 0.f ? kNegInf : (M + __log2f(L)) * (1.0f / kLog2e);
 }
 
 // 16-head tiles that share one pass over the keys: the whole group up to 64 heads (32 in fp32, whose fragments take

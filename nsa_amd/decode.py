@@ -282,6 +282,10 @@ class NSAPagedDecodeCache:
         if rc:
             _lib.check(rc, "nsa_paged_cache_move")
 
+    @staticmethod
+    def _ids(slots):
+        return slots.tolist() if isinstance(slots, torch.Tensor) else list(slots)
+
     def _check_slot(self, b):
         if not 0 <= b < self.batch:
             raise ValueError("slot %d of a cache of %d sequences" % (b, self.batch))
@@ -290,7 +294,7 @@ class NSAPagedDecodeCache:
         """The sequence of slot src continues in the slots dst (a slot or several) as well, or its first `length` tokens
         do; what dst held is released.  Full pages are shared, the partly filled last page and the compressed rows are
         copied, in one launch.  RuntimeError, and nothing changes, when the pool has no pages left for the copies."""
-        dst = [dst] if isinstance(dst, int) else list(dst)
+        dst = [dst] if isinstance(dst, int) else self._ids(dst)
         self._check_slot(src)
         length = self._lens[src] if length is None else length
         if not 0 <= length <= self._lens[src]:
@@ -301,8 +305,9 @@ class NSAPagedDecodeCache:
 
     def reorder(self, parents):
         """Slot b continues the sequence that slot parents[b] held, for every slot at once, as after a beam-search step; a
-        parent may come up several times or not at all.  Pages are shared and copied as by fork()."""
-        parents = list(parents)
+        parent may come up several times or not at all.  Pages are shared and copied as by fork().  (A tensor of parents on
+        the GPU is read back, which waits for it.)"""
+        parents = self._ids(parents)
         if len(parents) != self.batch:
             raise ValueError("reorder() got %d parents for %d slots" % (len(parents), self.batch))
         self._check_slot(min(parents))

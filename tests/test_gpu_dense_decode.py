@@ -152,6 +152,28 @@ def test_what_lies_behind_a_sequence_does_not_matter(paged, garbage, dtype):
     check(q, c, ks, vs, window=37)
 
 
+@pytest.mark.parametrize("cap", [256, 2048])                      # one launch, and the split schedule
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_nan_among_the_visible_comes_through(cap, dtype):
+    """a NaN in a query is its head's, in a key all heads' that read it, in a value one channel's; nobody else's"""
+    from nsa_amd.decode import dense_decode_step
+    lens = [200, cap, 130]
+    c, ks, vs = make_cache(True, lens, cap, 2, 64, 64, dtype, seed=55)
+    q = randn(3, 8, 64, seed=56, dtype=dtype).to(DEV)
+    want, want_lse = dense_decode_step(q, c, return_lse=True)
+    bad = q.clone()
+    bad[0, 1, 5] = math.nan
+    page = c.block_table[1, 1].long()
+    c.k_pool[page, 3, 1, 7] = math.nan
+    c.v_pool_t[c.block_table[2, 0].long(), 0, 9, 2] = math.nan
+    out, lse = dense_decode_step(bad, c, return_lse=True)
+    nan, nan_lse = torch.zeros_like(out, dtype=torch.bool), torch.zeros_like(lse, dtype=torch.bool)
+    nan[0, 1] = nan[1, 4:] = nan[2, :4, 9] = True
+    nan_lse[0, 1] = nan_lse[1, 4:] = True
+    assert torch.equal(out.isnan(), nan) and torch.equal(lse.isnan(), nan_lse)
+    assert torch.equal(out[~nan], want[~nan]) and torch.equal(lse[~nan_lse], want_lse[~nan_lse])
+
+
 def test_lowest_values_as_scores_and_large_scores():
     """Scores at the ends of the range: one key far above the others, and all of them equally low."""
     dtype = torch.float32
