@@ -85,14 +85,14 @@ def plain(q, k, v, scale, window):
     return out, lse, tol, tol_lse
 
 
-def check(q, c, ks, vs, window=0, scale=None, **kw):
+def check(q, c, ks, vs, window=0, scale=None, where="cpu", **kw):
     from nsa_amd.decode import dense_decode_step
     out, lse = dense_decode_step(q, c, scale=scale, sliding_window=window, return_lse=True, **kw)
     assert out.dtype == q.dtype and out.shape == (q.shape[0], q.shape[1], c.dv) and lse.shape == q.shape[:2]
     scale = q.shape[2] ** -0.5 if scale is None else scale
-    got, got_lse = out.double().cpu(), lse.double().cpu()
+    got, got_lse = out.double().to(where), lse.double().to(where)
     for b in range(len(ks)):
-        ref, ref_lse, tol, tol_lse = plain(q[b].cpu(), ks[b], vs[b], scale, window)
+        ref, ref_lse, tol, tol_lse = plain(q[b].to(where), ks[b], vs[b], scale, window)
         assert torch.isfinite(got[b]).all(), b
         assert ((got[b] - ref).abs() <= tol).all(), (b, len(ks[b]), float(((got[b] - ref).abs() / tol).max()))
         if len(ks[b]) == 0:
@@ -193,6 +193,25 @@ def test_many_sequences(paged):
     c, ks, vs = make_cache(paged, lens, 3008, 2, 64, 64, torch.bfloat16, seed=70)
     q = randn(len(lens), 16, 64, seed=69, dtype=torch.bfloat16).to(DEV)
     check(q, c, ks, vs)
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_random_shapes(seed):
+    """batch, lengths, capacity, heads, types, windows and scales drawn together"""
+    g = random.Random(1000 + seed)
+    dtype = g.choice([torch.bfloat16, torch.float16, torch.float32])
+    dk, dv = g.choice([(32, 32), (64, 64), (128, 128), (192, 128)])
+    hkv, group = g.choice([1, 2, 3, 5, 8]), g.choice([1, 2, 5, 8, 16, 20, 33, 64, 70])
+    B = g.choice([1, 2, 3, 9, 63, 64, 65, 130])
+    cap = g.choice([64, 128, 320, 1024, 1088, 2048] if B > 10 else [64, 192, 1024, 2048, 5056])
+    lens = [g.choice([g.randint(0, cap), cap, g.randint(0, min(cap, 130))]) for _ in range(B)]
+    window = g.choice([0, 0, 0, 1, 63, 64, 65, g.randint(1, cap)])
+    paged = g.random() < 0.6
+    c, ks, vs = make_cache(paged, lens, cap, hkv, dk, dv, dtype, seed=2000 + 300 * seed, garbage=g.choice([None, math.nan]))
+    q = randn(B, hkv * group, dk, seed=3000 + seed, dtype=dtype).to(DEV)
+    if B > 10:                                             # the reference runs on the GPU for the many
+        ks, vs = [k.to(DEV) for k in ks], [v.to(DEV) for v in vs]
+    check(q, c, ks, vs, window, g.choice([None, None, 0.05, -0.2]), where=DEV if B > 10 else "cpu")
 
 
 def test_units_of_more_pages_than_a_wavefront_has_lanes():

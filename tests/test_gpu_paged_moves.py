@@ -169,6 +169,70 @@ def test_truncate(n):
     check_books(c)
 
 
+@pytest.mark.parametrize("seed", range(8))
+def test_random_runs(seed):
+    """appends, fills, forks, reorders, cuts, releases and compactions one after the other, against the tokens every slot
+    should hold"""
+    rng = random.Random(seed)
+    kind = KINDS[seed % 4]
+    B = rng.choice([2, 5, 9, 20])
+    c = cache_of(B, 5 * B, 320, seed=seed, **kind)
+    dtype, n_new = c.k_pool.dtype, 0
+    want = [(torch.zeros(0, c.hkv, c.dk, dtype=dtype, device=DEV), torch.zeros(0, c.hkv, c.dv, dtype=dtype, device=DEV))
+            for _ in range(B)]
+
+    def fresh(*shape):
+        nonlocal n_new
+        n_new += 1
+        return randn(*shape, seed=10_000 * seed + n_new, dtype=dtype).to(DEV)
+
+    for step in range(60):
+        op = rng.choice(["append", "append", "fill", "fork", "reorder", "truncate", "release", "compact"])
+        before = [held(c, b) for b in range(B)]
+        try:
+            if op == "append":
+                for _ in range(rng.choice([1, 3, 40])):
+                    kn, vn = fresh(B, c.hkv, c.dk), fresh(B, c.hkv, c.dv)
+                    c.append(kn, vn)
+                    want = [(torch.cat([k, kn[b:b + 1]]), torch.cat([v, vn[b:b + 1]])) for b, (k, v) in enumerate(want)]
+            elif op == "fill":
+                b, n = rng.randrange(B), rng.choice([1, 64, 100, 200])
+                k, v = fresh(n, c.hkv, c.dk), fresh(n, c.hkv, c.dv)
+                c.fill(k, v, seq=b)
+                want[b] = (k, v)
+            elif op == "fork":
+                src = rng.randrange(B)
+                dst = rng.sample([b for b in range(B) if b != src], rng.randint(1, B - 1))
+                n = rng.choice([None, rng.randint(0, len(want[src][0]))])
+                c.fork(src, dst, n)
+                for b in dst:
+                    want[b] = (want[src][0][:n], want[src][1][:n])
+                    assert same(held(c, b), cut_to(c, before[src], len(want[src][0]) if n is None else n))
+            elif op == "reorder":
+                parents = rng.sample(range(B), B) if rng.random() < 0.5 else [rng.randrange(B) for _ in range(B)]
+                c.reorder(parents)
+                want = [want[p] for p in parents]
+                for b, p in enumerate(parents):
+                    assert same(held(c, b), before[p])
+            elif op == "truncate":
+                b = rng.randrange(B)
+                n = rng.randint(0, len(want[b][0]))
+                c.truncate(b, n)
+                want[b] = (want[b][0][:n], want[b][1][:n])
+                assert same(held(c, b), cut_to(c, before[b], n))
+            elif op == "release":
+                b = rng.randrange(B)
+                c.release(b)
+                want[b] = (want[b][0][:0], want[b][1][:0])
+            else:
+                c.compact()
+        except RuntimeError as e:
+            assert "exhausted" in str(e) or "capacity" in str(e)
+        for b in range(B):
+            assert same(held(c, b)[:2], want[b]), (step, op, b)
+        check_books(c)
+
+
 def test_exhausted_pool_changes_nothing():
     c = filled([100, 100, 0, 0], 128, pages=5)
     before = [held(c, b) for b in range(4)]

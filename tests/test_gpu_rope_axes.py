@@ -116,6 +116,48 @@ def test_many_rows(n):
     assert (d[:, at[3] + 3 * hq:] == 0).all()
 
 
+@pytest.mark.parametrize("seed", range(24))
+def test_random_layouts(seed):
+    """heads, head dims, rotary ranges, gaps, gate alignment, axes, types and row counts drawn together"""
+    import random
+    from nsa_amd import ops
+    g = random.Random(seed)
+    dtype = g.choice([torch.bfloat16, torch.float16, torch.float32])
+    interleaved = g.random() < 0.5
+    hq, hkv = g.randint(1, 20), g.randint(1, 6)
+    dk, dv = 8 * g.randint(2, 32), 8 * g.randint(1, 20)
+    unit = 8 if interleaved else 16
+    dim = unit * g.randint(1, dk // unit)
+    off = 8 * g.randint(0, (dk - dim) // 8)
+    axes, n = g.randint(1, 4), g.choice([1, 3, 17, 64, 129, 1500])
+    gap = 8 * g.choice([0, 0, 1, 3])
+    with_gates = g.random() < 0.8
+    at = [0, hq * dk + gap, hq * dk + hkv * dk + gap, hq * dk + hkv * (dk + dv) + gap + g.choice([0, 0, 3])]
+    ld = (at[3] + 3 * hq + 7) // 8 * 8 + 8 * g.choice([0, 2])
+    pair_axis = [g.randrange(axes) for _ in range(dim // 2)]
+    inv = freqs(dim // 2)
+    pos = far_positions(axes, n, seed).to(DEV)
+    packed = randn(n, ld, seed=seed, dtype=dtype)
+    kw = dict(inv_freq=inv, positions=pos, rope_off=off, rope_dim=dim, interleaved=interleaved, pair_axis=pair_axis)
+    q, k, v, gates = ops.qkv_rope_split(packed.to(DEV), hq, hkv, dk, dv, tuple(at), with_gates=with_gates, **kw)
+    close(q, *rotated(packed[:, :hq * dk].reshape(n, hq, dk), pos, pair_axis, inv, off, interleaved))
+    close(k, *rotated(packed[:, at[1]:at[1] + hkv * dk].reshape(n, hkv, dk), pos, pair_axis, inv, off, interleaved))
+    assert torch.equal(v.cpu().view(n, -1), packed[:, at[2]:at[2] + hkv * dv])
+    assert (gates is None) != with_gates
+    if with_gates:
+        assert torch.equal(gates.cpu().view(n, -1), packed[:, at[3]:at[3] + 3 * hq])
+    d = ops.qkv_rope_pack(q, k, v, gates, ld, tuple(at), **kw).cpu()
+    close(d[:, :hq * dk].reshape(n, hq, dk), *rotated(q.cpu(), pos, pair_axis, inv, off, interleaved, -1.0))
+    close(d[:, at[1]:at[1] + hkv * dk].reshape(n, hkv, dk), *rotated(k.cpu(), pos, pair_axis, inv, off, interleaved, -1.0))
+    assert torch.equal(d[:, at[2]:at[2] + hkv * dv], v.cpu().view(n, -1))
+    rest = torch.ones(ld, dtype=torch.bool)
+    for lo, w in ((0, hq * dk), (at[1], hkv * dk), (at[2], hkv * dv), (at[3], 3 * hq if with_gates else 0)):
+        rest[lo:lo + w] = False
+    assert (d[:, rest] == 0).all()
+    if with_gates:
+        assert torch.equal(d[:, at[3]:at[3] + 3 * hq], gates.cpu().view(n, -1))
+
+
 def test_positions_at_the_ends_of_their_range():
     from nsa_amd import ops
     hq, hkv, dk, dv, dim = 2, 1, 64, 64, 64
