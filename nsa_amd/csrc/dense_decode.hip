@@ -404,21 +404,24 @@ dense_decode_join_kernel(const DenseDecodeArgs a, int rows_per_slot, int blocks)
 }
 
 // 16-head tiles that share one pass over the keys: the whole group up to 64 heads (32 in fp32, whose fragments take
-// twice the registers); larger groups read the keys once per block.
-static int dense_tiles(const DenseDecodeArgs& a) {
+// twice the registers); larger groups read the keys once per block.  Four tiles leave one wavefront per SIMD and join in
+// four rounds, so where there are few pages blocks of two are faster, although both read them (64 / 1 heads of 128 bf16,
+// four tiles against two: 2 sequences of 8192 tokens 20.5 and 15.3 us, 2 of 32768 28.1 and 23.7, 16 of 32768 97 and 103;
+// 192 / 128: 22.1 and 17.4, 30.2 and 29.0, 96 and 148).
+static int dense_tiles(const DenseDecodeArgs& a, long pages) {
   const int G = a.hq / a.hkv;
   if (G <= 16) return 1;
-  return G <= 32 || a.dtype == 1 ? 2 : 4;
+  return G <= 32 || a.dtype == 1 || pages * a.hkv <= 1024 ? 2 : 4;
 }
 
 DensePlan dense_decode_plan(const DenseDecodeArgs& a) {
   DensePlan p;
   const int G = a.hq / a.hkv;
-  p.tiles = dense_tiles(a);
-  p.blocks = (G + 16 * p.tiles - 1) / (16 * p.tiles);
-  const long per = (long)a.hkv * p.blocks;
   const int cap_pages = (a.ctx_cap + 63) / 64;
   const int span = a.window > 0 ? (int)min((long)cap_pages, ((long)a.window + 62) / 64 + 1) : cap_pages;
+  p.tiles = dense_tiles(a, (long)a.batch * span);
+  p.blocks = (G + 16 * p.tiles - 1) / (16 * p.tiles);
+  const long per = (long)a.hkv * p.blocks;
   // One workgroup per CU where its four wavefronts keep 64 KB of loads in flight, more where a chunk is smaller: few long
   // streams reach more of the memory's rate than many (64 sequences of 32768 tokens, 128 / 128 bf16: 722 us with 256
   // workgroups, 767 with 512, 791 with 768; 16 of them at 64 / 64: 108, 102, 105 us)

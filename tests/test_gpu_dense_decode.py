@@ -125,9 +125,10 @@ def test_every_length(paged, dtype, hq, hkv, dk, dv, window):
 @pytest.mark.parametrize("dtype,dk,dv", [(torch.bfloat16, 128, 128), (torch.float32, 64, 64), (torch.bfloat16, 192, 128),
                                          (torch.float32, 192, 128)])
 @pytest.mark.parametrize("group", [1, 2, 3, 7, 15, 16, 17, 24, 32, 33, 48, 64, 65, 80, 130])
-def test_every_group_size(dtype, dk, dv, group):
+@pytest.mark.parametrize("cap", [320, 12800])          # beyond 1024 pages per call a group of up to 64 heads stays together
+def test_every_group_size(cap, dtype, dk, dv, group):
     lens = [300, 77, 1]
-    c, ks, vs = make_cache(True, lens, 320, 2, dk, dv, dtype, seed=30)
+    c, ks, vs = make_cache(True, lens, cap, 2, dk, dv, dtype, seed=30)
     q = randn(len(lens), 2 * group, dk, seed=29, dtype=dtype).to(DEV)
     check(q, c, ks, vs)
 
