@@ -482,7 +482,8 @@ int nsa_dense_decode_step(const void* q, const void* k_cache, const void* v_cach
  * NSA_ERR_INVALID or NSA_ERR_RESOURCE (not enough free pages) with nothing changed.
  * nsa_paged_cache_grow (host) gives a slot pages from the free list until it holds `pages` of them, all or nothing.
  * nsa_paged_cache_move carries the moves out on the device (`moves` is a HOST pointer, read during the call): page table,
- * ctx_lens, last pages and compressed rows (block / stride as the cache was built), in one launch per 80 moves.
+ * ctx_lens, last pages and compressed rows (block / stride as the cache was built), in one launch per 80 moves.  A move with
+ * dst -1 puts a slot into a register and the next one with src -1 writes it: at most 79 moves later (the plan's are).
  * nsa_paged_cache_compact_plan (host) / nsa_paged_cache_compact_move (device; `pairs`, up to num_pages (page, new page)
  * pairs, is a HOST pointer): moves pages down until the pages in use are 1 .. *used.  No counterpart in the reference. */
 int nsa_paged_cache_plan(int32_t* table, int32_t* lens, int32_t* held, int32_t* refs, int32_t* free_pages, int32_t* n_free,

@@ -970,15 +970,18 @@ int nsa_paged_cache_move(void* k_pool, void* v_pool_t, int32_t* block_table, voi
       block <= 0 || stride <= 0)
     return fail(NSA_ERR_INVALID, "paged_cache_move: sizes must be positive and nc_cap a multiple of 64");
   if (!aligned16(ck_cache) || !aligned16(cv_cache_t)) return fail(NSA_ERR_INVALID, "paged_cache_move: pointers must be 16-byte aligned");
-  bool kept = false;                     // whether the register holds a slot
+  int kept = -1;                         // the move that put a slot into the register, while it is there
   for (int i = 0; i < n_moves; ++i) {
     const int32_t* m = moves + 5L * i;
     if (m[0] < -1 || m[0] >= batch || m[1] < -1 || m[1] >= batch || m[2] < 0 || m[2] > max_pages * 64 || m[3] < 0 ||
-        m[3] >= num_pages || m[4] < 0 || m[4] >= num_pages || (m[1] < 0 && (kept || m[0] < 0)) || (m[0] < 0 && !kept))
+        m[3] >= num_pages || m[4] < 0 || m[4] >= num_pages || (m[1] < 0 && (kept >= 0 || m[0] < 0)) || (m[0] < 0 && kept < 0))
       return fail(NSA_ERR_INVALID, "paged_cache_move: move %d names a slot, length or page outside the cache", i);
-    if (m[1] < 0) kept = true;
-    else if (m[0] < 0) kept = false;
+    if (m[1] < 0) kept = i;
+    if (kept >= 0 && i - kept >= nsa::kPagedMoves)
+      return fail(NSA_ERR_INVALID, "paged_cache_move: the moves %d .. %d keep the register for more than a launch", kept, i);
+    if (m[0] < 0) kept = -1;
   }
+  if (kept >= 0) return fail(NSA_ERR_INVALID, "paged_cache_move: move %d leaves the register full", kept);
   if (n_moves == 0) return NSA_OK;
   a.block_table = block_table; a.ck = ck_cache; a.cv = cv_cache_t; a.ctx_lens = ctx_lens;
   a.max_pages = max_pages; a.hkv = hkv; a.dk = dk; a.dv = dv; a.nc_cap = nc_cap;

@@ -390,6 +390,11 @@ def test_paged_move_argument_errors_do_not_launch(lib):
                 dict(moves=moves(-1, 1, 70, 1, 2)), dict(moves=moves(-1, -1, 70, 1, 2)),
                 dict(moves=moves(0, -1, 70, 1, 2, 1, -1, 70, 1, 2), n=2)):
         assert call(**bad) == -1, bad
+    # the register has to be read again, and within a launch
+    assert call(moves=moves(0, -1, 70, 1, 2)) == -1
+    assert call(moves=moves(0, 1, 70, 1, 2, 1, -1, 70, 1, 2), n=2) == -1
+    long = (ctypes.c_int32 * 500)(*([0, -1, 64, 0, 0] + [0, 1, 64, 0, 0] * 79 + [-1, 1, 64, 0, 0]))
+    assert call(moves=long, n=81) == -1
     assert call(dk=60) == -2 and call(n=0, moves=None) == 0
     comp = [p, p, p, moves(9, 1), 1, 2, 4, 8, 2, 64, 64, 0, None]
     assert lib.nsa_paged_cache_compact_move(*comp) == -1
