@@ -84,6 +84,12 @@ __device__ __forceinline__ int dense_unit_pages(const DenseDecodeArgs& a) {
   return C;
 }
 
+// How far below the running maximum the reference of the exponentials lies.  float16 ends at 2^-24: with probabilities of up
+// to 2^(7 + 8) instead of 1 it keeps what lies 2^-31 below the maximum, which thousands of such keys add up to (one key
+// that takes nearly all the weight, 1000 others at 2^-26 each: 1/8 of their sum was lost without).
+template <typename T> constexpr float kDenseBelow = 0.0f;
+template <> constexpr float kDenseBelow<f16_t> = 7.0f;
+
 // Fragments of one 32-key chunk and the two products on them.  Visible keys of the chunk [cb, cb + 32) are lo..n-1.
 // Whatever a page holds outside them (rows of a sequence that had the page before, infinities, NaN) must not reach the
 // sums: their scores are replaced, and their values too, since 0 * inf is NaN.
@@ -127,10 +133,11 @@ __device__ __forceinline__ void dense_values(DecState<T, DK, DV> (&st)[NT], vec8
       mx = fmaxf(mx, whole || (key >= lo && key < n) ? x : kNegInf);
     }
     // The reference of the exponentials follows the maximum only when that has grown by more than 2^8 (the first chunk, and
-    // hardly ever again): probabilities stay below 2^8, and the sums are not rescaled at every chunk.
+    // hardly ever again): probabilities stay below 2^8 (float16: 2^15), and the sums are not rescaled at every chunk.
     mx = colgroup_max(mx);
-    if (__any(mx > st[j].m + kMaxSlackLog2)) {
-      const float m_new = fmaxf(st[j].m, mx);
+    constexpr float below = kDenseBelow<T>;
+    if (__any(mx > st[j].m + (kMaxSlackLog2 + below))) {
+      const float m_new = fmaxf(st[j].m, mx - below);
       const float alpha = fast_exp2(st[j].m - (m_new == kNegInf ? 0.f : m_new));
       st[j].m = m_new;
       st[j].l *= alpha;

@@ -371,3 +371,31 @@ def test_captured_calls_follow_the_growing_cache():
     for b in range(B):
         ref, _, tol, _ = plain(q[-1, b].cpu(), k[b].cpu(), v[b].cpu(), D ** -0.5, 0)
         assert ((outs[0][b].double().cpu() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("lens,cap,hq,hkv", [([1000, 997], 1024, 4, 1), ([2000] * 64, 2048, 8, 4), ([1500] * 40, 2048, 64, 1)])
+def test_float16_keeps_what_lies_far_below_the_maximum(lens, cap, hq, hkv):
+    """One key takes almost all of the weight and has a value of zero, so the output is the sum of the others' weights of
+    e^-18.06 = 2^-26.06 each: below the last step of float16 beside a maximum of 1, and held beside one of 2^7.  A wavefront's
+    probability is off by 2^-25 at most where float16 ends, the denominator then is at least 2^7 in the same units, hence
+    2^-32 n max |v| in the place of the bound's last term."""
+    from nsa_amd.decode import dense_decode_step
+    dk = dv = 32
+    c, ks, vs = make_cache(False, lens, cap, hkv, dk, dv, torch.float16, seed=140)
+    for k, v in zip(ks, vs):
+        k.zero_()
+        k[0, :, 0] = 4.25
+        v.fill_(1024.0)
+        v[0] = 0.0
+    for b, n in enumerate(lens):
+        c.k[b, :n] = ks[b].to(DEV)
+        c.vt[b, :, :, :n] = vs[b].permute(1, 2, 0).to(DEV)
+    q = torch.zeros(len(lens), hq, dk, dtype=torch.float16)
+    q[:, :, 0] = 4.25
+    out, lse = dense_decode_step(q.to(DEV), c, scale=1.0, return_lse=True)
+    for b, n in enumerate(lens):
+        ref, ref_lse, tol, tol_lse = plain(q[b], ks[b], vs[b], 1.0, 0)
+        tol = tol + (2.0 ** -32 - 2.0 ** -25) * n * 1024.0
+        err = (out[b].double().cpu() - ref).abs()
+        assert (err <= tol).all(), (b, float((err / tol).max()))
+        assert ((lse[b].double().cpu() - ref_lse).abs() <= tol_lse).all()
