@@ -225,12 +225,10 @@ class NSAPagedDecodeCache:
         if T > self.ctx_cap:
             raise RuntimeError(f"sequence {seqs[0]} would exceed the cache capacity of {self.ctx_cap} tokens")
         entries = []
-        if self._shares:
-            for b in seqs:
-                self.release(b)
-        for b in seqs:
+        for b in reversed(seqs):         # all of them before any grows: the pages of one may be needed by another
             if self._lens[b]:
                 self.release(b)
+        for b in seqs:
             entries += [(b, slot, pg) for slot, pg in self._grow(b, T)]
             self._lens[b] = T
         self._publish(entries)

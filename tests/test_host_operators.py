@@ -468,3 +468,42 @@ def test_a_copy_of_a_cache_has_books_of_its_own():
     assert d.free_pages == 6 and c.free_pages == 4 and c._lens[0] == 70
     Model(d).append(1, 30)
     assert c._held[1] == 0 and d._held[1] == 1
+
+
+def uneven_full_pool(shared=False):
+    """4 pages: slot 0 holds one of them, slot 2 the other three (compression blocks of 64: fill() of fewer tokens runs on
+    the CPU)."""
+    from nsa_amd.decode import NSAPagedDecodeCache
+    c = NSAPagedDecodeCache(3, 4, 192, 1, 8, 8, block=64, dtype=torch.float32, device="cpu")
+    c.fill(torch.ones(30, 1, 8), torch.ones(30, 1, 8), seq=0)
+    c._publish([(2, s, p) for s, p in c._grow(2, 190)])
+    c._lens[2] = 190
+    c.ctx_lens[2] = 190
+    c._shares = shared
+    return c
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_fill_takes_the_pages_of_every_slot_it_refills(shared):
+    """a full pool whose pages sit in the last slot: all slots are refilled, and both sides of the books agree"""
+    c = uneven_full_pool(shared)
+    k, v = torch.randn(3, 60, 1, 8), torch.randn(3, 60, 1, 8)
+    c.fill(k, v)
+    assert list(c._lens) == c.ctx_lens.tolist() == [60] * 3 and list(c._held) == [1] * 3 and c.free_pages == 1
+    assert c.block_table.flatten().tolist() == list(c._table)
+    pages = [c._pages_of(b)[0] for b in range(3)]
+    assert len(set(pages)) == 3 and 0 not in pages and sorted(c._refs) == [0, 0, 1, 1, 1]
+    for b, p in enumerate(pages):
+        assert torch.equal(c.k_pool[p, :60], k[b]) and torch.equal(c.v_pool_t[p, :, :, :60], v[b].permute(1, 2, 0))
+    assert (c.k_pool[0] == 0).all()
+    c.fill(k[:, :0], v[:, :0])
+    assert c.free_pages == 4 and (c.block_table == 0).all() and (c.ctx_lens == 0).all()
+
+
+def test_fill_that_does_not_fit_changes_nothing():
+    c = uneven_full_pool()
+    before = books(c), c.block_table.clone(), c.ctx_lens.clone()
+    for T, what in ((65, "exhausted"), (193, "exhausted")):
+        with pytest.raises(RuntimeError, match=what):
+            c.fill(torch.zeros(3, T, 1, 8), torch.zeros(3, T, 1, 8))
+    assert before[0] == books(c) and torch.equal(before[1], c.block_table) and torch.equal(before[2], c.ctx_lens)
