@@ -86,6 +86,13 @@ class _FreePages:
     def __len__(self):
         return self.n.value
 
+    def __getstate__(self):          # ctypes arrays can be copied but not pickled
+        return list(self.ids), self.n.value
+
+    def __setstate__(self, state):
+        ids, n = state
+        self.ids, self.n = (C.c_int32 * len(ids))(*ids), C.c_int32(n)
+
     def _at(self, i):
         if not -self.n.value <= i < self.n.value:
             raise IndexError("free page %d of %d" % (i, self.n.value))
@@ -115,6 +122,7 @@ class NSAPagedDecodeCache:
     used by one thread and one stream at a time."""
 
     PAGE = 64
+    _BOOKS = ("_table", "_lens", "_held", "_refs")       # arrays that the library shares
 
     def __init__(self, batch, num_pages, max_ctx, hkv, dk, dv, block=32, stride=16, dtype=torch.bfloat16,
                  device="cuda"):
@@ -146,6 +154,17 @@ class NSAPagedDecodeCache:
     @property
     def free_pages(self) -> int:
         return len(self._free)
+
+    def __getstate__(self):
+        state = self.__dict__.copy()
+        for name in self._BOOKS:
+            state[name] = list(state[name])
+        return state
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        for name in self._BOOKS:
+            setattr(self, name, (C.c_int32 * len(state[name]))(*state[name]))
 
     def _books(self):
         return (self._table, self._lens, self._held, self._refs, self._free.ids, C.byref(self._free.n), self.batch,

@@ -507,3 +507,30 @@ def test_fill_that_does_not_fit_changes_nothing():
         with pytest.raises(RuntimeError, match=what):
             c.fill(torch.zeros(3, T, 1, 8), torch.zeros(3, T, 1, 8))
     assert before[0] == books(c) and torch.equal(before[1], c.block_table) and torch.equal(before[2], c.ctx_lens)
+
+
+def test_a_pickled_cache_comes_back_with_its_books(tmp_path):
+    import pickle
+    c = small_cache(3, 9)
+    m = Model(c)
+    m.append(0, 130)
+    carry_out(c, plan_of(c, [1], [0], [100]))
+    m.tokens[1] = m.tokens[0][:100]
+    c.extra = "kept"
+    torch.save(c, tmp_path / "cache.pt")
+    for d in (pickle.loads(pickle.dumps(c)), torch.load(tmp_path / "cache.pt", weights_only=False)):
+        assert books(d) == books(c) and d.extra == "kept" and type(d._table) is type(c._table)
+        n = Model(d)
+        n.tokens, n.next = [list(t) for t in m.tokens], m.next
+        n.check()
+        n.append(2, 70)
+        d.release(0)
+        n.tokens[0] = []
+        n.check()
+        m.check()
+
+
+def plan_of(c, slots, parents, lengths):
+    moves, n = c._plan(slots, parents, lengths)
+    c._shares = True
+    return [tuple(moves[5 * i:5 * i + 5]) for i in range(n)]
