@@ -465,7 +465,8 @@ int nsa_decode_step_split_static(const void* q, const void* k_cache, const void*
  * workspace depend on the arguments alone and a captured call stays right while the sequences grow.  The result of a
  * sequence depends on where it is cut, hence to rounding on the other lengths of the batch; equal calls give equal bits.
  * workspace: nsa_dense_decode_workspace_bytes (0 for short capacities; ctx_cap = 64 * max_pages when paged; -1 for
- * invalid sizes); calls that share it must not overlap.  No counterpart in the reference, which has no cache. */
+ * invalid sizes); calls that share it must not overlap.  out, lse and the workspace must not overlap one another or
+ * anything that is read (NSA_ERR_INVALID).  No counterpart in the reference, which has no cache. */
 int64_t nsa_dense_decode_workspace_bytes(int batch, int hq, int hkv, int dk, int dv, int ctx_cap, int window, int dtype);
 int nsa_dense_decode_step(const void* q, const void* k_cache, const void* v_cache_t, const int32_t* block_table,
                           int max_pages, int num_pages, const int32_t* ctx_lens, void* out, float* lse, int batch, int hq,

@@ -854,6 +854,11 @@ static bool finite_bits(float x) {
   memcpy(&u, &x, sizeof(u));
   return (u & 0x7f800000u) != 0x7f800000u;
 }
+// Whether the bytes [a, a + na) and [b, b + nb) share any; null shares none.
+static bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && (x < y ? (int64_t)(y - x) < na : (int64_t)(x - y) < nb);
+}
 static bool dense_sizes_ok(int batch, int hq, int hkv, int ctx_cap, int window) {
   return batch > 0 && hq > 0 && hkv > 0 && hq % hkv == 0 && ctx_cap > 0 && ctx_cap <= 1 << 30 && ctx_cap % 64 == 0 && window >= 0 &&
          (int64_t)batch * (ctx_cap / 64) <= 0x7fffffff;
@@ -887,6 +892,17 @@ int nsa_dense_decode_step(const void* q, const void* k_cache, const void* v_cach
   const int64_t need = nsa::dense_decode_workspace_bytes(a);
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return fail(NSA_ERR_INVALID, "dense_decode: workspace missing, misaligned or smaller than nsa_dense_decode_workspace_bytes");
+  if (!nsa::dense_decode_dims_ok(dk, dv)) return finish(-2, "dense_decode");
+  // workgroups still read the operands when others write their results
+  const int64_t elem = dtype == NSA_F32 ? 4 : 2, tokens = block_table ? 64 * (int64_t)num_pages : (int64_t)batch * ctx_cap;
+  const struct { const void* p; int64_t bytes; } all[] = {
+      {out, (int64_t)batch * hq * dv * elem}, {lse, (int64_t)batch * hq * 4}, {need > 0 ? workspace : nullptr, need},
+      {q, (int64_t)batch * hq * dk * elem}, {k_cache, tokens * hkv * dk * elem}, {v_cache_t, tokens * hkv * dv * elem},
+      {ctx_lens, (int64_t)batch * 4}, {block_table, (int64_t)batch * max_pages * 4}};
+  for (int i = 0; i < 3; ++i)            // out, lse and the workspace are written
+    for (int j = i + 1; j < 8; ++j)
+      if (overlap(all[i].p, all[i].bytes, all[j].p, all[j].bytes))
+        return fail(NSA_ERR_INVALID, "dense_decode: out, lse and the workspace must not overlap one another, the query or the cache");
   const int rc = nsa::launch_dense_decode(a, workspace, stream);
   if (rc == -5) return fail(NSA_ERR_UNSUPPORTED, "dense_decode: more than 2^31-1 workgroups");
   return finish(rc, "dense_decode");

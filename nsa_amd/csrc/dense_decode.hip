@@ -457,6 +457,11 @@ long dense_decode_workspace_bytes(const DenseDecodeArgs& a) {
   return p.split ? p.slots * p.rows * (long)(a.dv + 2) * (long)sizeof(float) : 0;
 }
 
+// The head dims that launch_dense builds.
+bool dense_decode_dims_ok(int dk, int dv) {
+  return (dk == dv && (dk == 32 || dk == 64 || dk == 128)) || (dk == 192 && dv == 128);
+}
+
 template <typename T, int DK, int DV, int NT>
 static int launch_dense_n(const DenseDecodeArgs& a, const DensePlan& p, hipStream_t st) {
   const long units = p.split ? (long)p.units + a.batch : a.batch;

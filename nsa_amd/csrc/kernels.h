@@ -152,6 +152,7 @@ struct DenseDecodeArgs {
 struct DensePlan { int tiles, blocks, units, rows; long slots; bool whole, split; };
 DensePlan dense_decode_plan(const DenseDecodeArgs& a);
 long dense_decode_workspace_bytes(const DenseDecodeArgs& a);
+bool dense_decode_dims_ok(int dk, int dv);
 int launch_dense_decode(DenseDecodeArgs a, void* workspace, hipStream_t st);
 
 // Forks and moves in the paged cache (paged_cache.hip).  Host bookkeeping, owned by the caller: the page table, the tokens

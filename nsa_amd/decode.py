@@ -533,7 +533,8 @@ def dense_decode_step(q: torch.Tensor, cache, scale: Optional[float] = None, sli
 
     The tokens of all sequences are cut into equal pieces from the lengths on the device: few long sequences fill the
     card, a ragged batch does not wait for its longest, and a captured call stays right while the sequences grow.
-    out [B,Hq,Dv] / lse float32 [B,Hq]: result buffers of the caller (allocated here when None)."""
+    out [B,Hq,Dv] / lse float32 [B,Hq]: result buffers of the caller (allocated here when None), which must not overlap
+    each other, q or the cache."""
     _need_cuda(q)
     B, hkv, dv, paged = cache.batch, cache.hkv, cache.dv, isinstance(cache, NSAPagedDecodeCache)
     if q.dim() != 3 or q.shape[0] != B or q.shape[2] != cache.dk:
@@ -557,8 +558,6 @@ def dense_decode_step(q: torch.Tensor, cache, scale: Optional[float] = None, sli
     elif out.shape != (B, hq, dv) or out.dtype != q.dtype or out.device != device or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise ValueError("out must be a contiguous, 16-byte aligned [B,Hq,Dv] tensor of q's dtype and device")
-    if out.data_ptr() == q.data_ptr():
-        raise ValueError("out must not be q: workgroups still read the query when others write")
     if lse is None:
         if return_lse:
             lse = torch.empty((B, hq), dtype=torch.float32, device=device)

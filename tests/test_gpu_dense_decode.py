@@ -399,3 +399,24 @@ def test_float16_keeps_what_lies_far_below_the_maximum(lens, cap, hq, hkv):
         err = (out[b].double().cpu() - ref).abs()
         assert (err <= tol).all(), (b, float((err / tol).max()))
         assert ((lse[b].double().cpu() - ref_lse).abs() <= tol_lse).all()
+
+
+def test_results_that_overlap_the_operands_are_refused():
+    """out or lse inside another operand's memory, at its start or later; right behind it they may lie"""
+    from nsa_amd.decode import dense_decode_step
+    c, ks, vs = make_cache(True, [500, 3], 512, 2, 64, 64, torch.bfloat16, seed=117)
+    n = 2 * 8 * 64
+    pool = torch.zeros(4 * n, dtype=torch.bfloat16, device=DEV)
+    q = pool[n:2 * n].view(2, 8, 64)
+    q.copy_(randn(2, 8, 64, seed=118, dtype=torch.bfloat16))
+    out_at = lambda i: pool[i:i + n].view(2, 8, 64)                                     # noqa: E731
+    lse_at = lambda i: pool[i:i + 32].view(torch.float32).view(2, 8)                    # noqa: E731
+    for bad in (dict(out=out_at(n)), dict(out=out_at(n + 8)), dict(out=out_at(8)), dict(out=out_at(2 * n - 8)),
+                dict(lse=lse_at(n)), dict(lse=lse_at(2 * n - 32)), dict(out=out_at(2 * n), lse=lse_at(3 * n - 32)),
+                dict(out=c.k_pool.view(-1)[-n:].view(2, 8, 64)), dict(out=c.v_pool_t.view(-1)[:n].view(2, 8, 64)),
+                dict(lse=c.block_table.view(torch.float32).view(-1)[:16].view(2, 8))):
+        with pytest.raises(ValueError, match="overlap"):
+            dense_decode_step(q, c, **bad)
+    want, _ = check(q, c, ks, vs)
+    got, _ = check(q, c, ks, vs, out=out_at(2 * n), lse=lse_at(3 * n))
+    assert torch.equal(got, want) and torch.equal(dense_decode_step(q, c, out=out_at(0)), want)

@@ -534,3 +534,33 @@ def plan_of(c, slots, parents, lengths):
     moves, n = c._plan(slots, parents, lengths)
     c._shares = True
     return [tuple(moves[5 * i:5 * i + 5]) for i in range(n)]
+
+
+def test_dense_decode_refuses_results_on_top_of_its_operands(lib):
+    """made-up addresses, far apart but for the pair under test: every call is refused before a launch"""
+    names = ["q", "k", "v", "table", "max_pages", "num_pages", "lens", "out", "lse", "batch", "hq", "hkv", "dk", "dv", "cap",
+             "window", "scale", "dtype", "ws", "ws_bytes", "stream"]
+    B, hq, hkv, dk, dv, pages, width = 2, 16, 2, 64, 64, 8, 64
+    gap = 1 << 32
+    at = {n: (i + 1) * gap for i, n in enumerate(["q", "k", "v", "table", "lens", "out", "lse", "ws"])}
+    need = lib.nsa_dense_decode_workspace_bytes(B, hq, hkv, dk, dv, 64 * width, 0, 0)
+    size = dict(q=B * hq * dk * 2, k=pages * 64 * hkv * dk * 2, v=pages * 64 * hkv * dv * 2, table=B * width * 4, lens=B * 4,
+                out=B * hq * dv * 2, lse=B * hq * 4, ws=need)
+    good = dict(at, max_pages=width, num_pages=pages, batch=B, hq=hq, hkv=hkv, dk=dk, dv=dv, cap=0, window=0, scale=0.1,
+                dtype=0, ws_bytes=need, stream=None)
+
+    def refused(**kw):
+        assert lib.nsa_dense_decode_step(*[dict(good, **kw)[n] for n in names]) == -1, kw
+        return b"overlap" in lib.nsa_last_error_string()
+
+    for result in ("out", "lse", "ws"):
+        for other in at:
+            if other == result:
+                continue
+            for where in (at[other], at[other] + (size[other] - 1) // 16 * 16, at[other] - (size[result] - 1) // 16 * 16):
+                assert refused(**{result: where}), (result, other, where - at[other])
+    # a contiguous cache reaches over the whole capacity
+    last = at["k"] + B * 64 * width * hkv * dk * 2 - 16
+    assert refused(table=None, cap=64 * width, max_pages=0, num_pages=0, out=last)
+    # its type decides how far an operand reaches
+    assert refused(dtype=1, ws_bytes=1 << 31, out=at["q"] + B * hq * dk * 2)
