@@ -15,6 +15,8 @@
 // wavefront computes the same plan from them, so that a captured graph stays right as the sequences grow; the host
 // only fixes an upper bound of the number of units.  A sequence of more than one unit leaves one partial softmax
 // state (fp32) per unit, and a second kernel joins them; the others are finished by the first kernel.
+#include <type_traits>
+
 #include "decode_common.h"
 
 namespace nsa {
@@ -90,6 +92,12 @@ __device__ __forceinline__ int dense_unit_pages(const DenseDecodeArgs& a) {
 template <typename T> constexpr float kDenseBelow = 0.0f;
 template <> constexpr float kDenseBelow<f16_t> = 7.0f;
 
+// A 16-bit value that is no number or infinite, by its bits (the library is compiled with the promise that no NaN occurs).
+template <typename T> constexpr unsigned kExpMask16 = 0x7f80u;
+template <> constexpr unsigned kExpMask16<f16_t> = 0x7c00u;
+template <typename T>
+__device__ __forceinline__ bool odd16(T x) { return (__builtin_bit_cast(uint16_t, x) & kExpMask16<T>) == kExpMask16<T>; }
+
 // Fragments of one 32-key chunk and the two products on them.  Visible keys of the chunk [cb, cb + 32) are lo..n-1.
 // Whatever a page holds outside them (rows of a sequence that had the page before, infinities, NaN) must not reach the
 // sums: their scores are replaced, and their values too, since 0 * inf is NaN.
@@ -108,9 +116,12 @@ __device__ __forceinline__ void dense_scores(const vec8_t<T> (&k0)[DK / 32], con
     for (int i = 0; i < 4; ++i) { s[j][i] = s0[i]; s[j][4 + i] = s1[i]; }
   }
 }
-template <typename T, int DK, int DV, int NT>
+// ODD: among the values there are infinities or NaN, which the split probabilities would turn into NaN (infinity times a
+// rest of 0, or of the other sign).  The keys are gone through twice then: with the finite values alone (`finite`), and with
+// the others alone, each with weight 1 unless its probability is 0.
+template <bool ODD, typename T, int DK, int DV, int NT>
 __device__ __forceinline__ void dense_values(DecState<T, DK, DV> (&st)[NT], vec8_t<T> (&v)[DV / 16],
-                                             const float (&s)[NT][8], int cb, int lo, int n, float c, int g) {
+                                             const float (&s)[NT][8], int cb, int lo, int n, float c, int g, bool finite) {
   const bool whole = cb >= lo && cb + 32 <= n;
   if (!whole) {
 #pragma unroll
@@ -121,6 +132,13 @@ __device__ __forceinline__ void dense_values(DecState<T, DK, DV> (&st)[NT], vec8
         for (int t = 0; t < DV / 16; ++t) v[t][i] = (T)0.0f;
       }
     }
+  }
+  if constexpr (ODD) {
+#pragma unroll
+    for (int t = 0; t < DV / 16; ++t)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (odd16<T>(v[t][i]) == finite) v[t][i] = (T)0.0f;
   }
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
@@ -153,9 +171,10 @@ __device__ __forceinline__ void dense_values(DecState<T, DK, DV> (&st)[NT], vec8
       const int key = cb + 8 * g + i;
       const float x = fast_exp2(fmaf(s[j][i], c, -mref));
       p[i] = whole || (key >= lo && key < n) ? x : 0.f;
+      if (ODD && !finite) p[i] = p[i] == 0.f ? 0.f : 1.f;
       sum += p[i];
     }
-    st[j].l += sum;
+    if (!ODD || finite) st[j].l += sum;
     // The second product takes 16-bit probabilities: a rounded one and what the rounding left, each with its own matrix
     // instructions (the loads are the bound), so that only the rounding of the result remains.
     const vec8_t<T> pb = pack8<T>(p);
@@ -167,7 +186,9 @@ __device__ __forceinline__ void dense_values(DecState<T, DK, DV> (&st)[NT], vec8
 #pragma unroll
     for (int t = 0; t < DV / 16; ++t) {
       st[j].o[t] = mma16(v[t], pb, st[j].o[t]);
-      if constexpr (sizeof(T) == 2) st[j].o[t] = mma16(v[t], rest, st[j].o[t]);
+      if constexpr (sizeof(T) == 2) {
+        if (!ODD || finite) st[j].o[t] = mma16(v[t], rest, st[j].o[t]);
+      }
     }
   }
 }
@@ -215,57 +236,62 @@ dense_decode_kernel(const DenseDecodeArgs a) {
   const DenseSpan sp = dense_span(a.ctx_lens[b], a.ctx_cap, a.window);
   const int p0 = sp.first + idx * C, p1 = min(sp.first + sp.pages, p0 + C);
 
-  const T* kbase = reinterpret_cast<const T*>(a.k) + (long)h * DK + 8 * g;
-  const T* vbase = reinterpret_cast<const T*>(a.v);
-  const long krow = (long)a.hkv * DK;
-  const bool paged = a.block_table != nullptr;
-  const long vrow = paged ? 64 : a.ctx_cap;
-  const int32_t* table = paged ? a.block_table + (long)b * a.max_pages : nullptr;
-
-  vec8_t<T> q[NT][DK / 32];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int head = h * G + min(row0 + 16 * j + n16, G - 1);
-    const T* qp = reinterpret_cast<const T*>(a.q) + ((long)b * a.hq + head) * DK + 8 * g;
-#pragma unroll
-    for (int kk = 0; kk < DK / 32; ++kk) q[j][kk] = load8(qp + 32 * kk);
-  }
   DecState<T, DK, DV> st[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) dec_reset(st[j]);
-  const float c = a.scale * kLog2e;
 
-  // chunk i of this wavefront covers keys 64 p0 + 32 (w + 4 i) ..; 64 page ids at a time sit in the lanes
-  int ids_at = p0, ids = 0;
-  if (paged && p0 + lane < p1) ids = table[p0 + lane];
-  auto page_of = [&](int cb) -> int {
-    const int p = cb >> 6;
-    if (p - ids_at >= 64) {
-      ids_at = p;
-      ids = p + lane < p1 ? table[p + lane] : 0;
+  // one run over this wavefront's chunks of the unit
+  auto stream = [&](auto odd, bool finite, int lane) {
+    constexpr bool kOdd = decltype(odd)::value;
+    const int n16 = lane & 15, g = lane >> 4;
+    const T* kbase = reinterpret_cast<const T*>(a.k) + (long)h * DK + 8 * g;
+    const T* vbase = reinterpret_cast<const T*>(a.v);
+    const long krow = (long)a.hkv * DK;
+    const bool paged = a.block_table != nullptr;
+    const long vrow = paged ? 64 : a.ctx_cap;
+    const int32_t* table = paged ? a.block_table + (long)b * a.max_pages : nullptr;
+
+    vec8_t<T> q[NT][DK / 32];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int head = h * G + min(row0 + 16 * j + n16, G - 1);
+      const T* qp = reinterpret_cast<const T*>(a.q) + ((long)b * a.hq + head) * DK + 8 * g;
+#pragma unroll
+      for (int kk = 0; kk < DK / 32; ++kk) q[j][kk] = load8(qp + 32 * kk);
     }
-    // an id outside the pool would fault: read page 0 instead (the caller's table is wrong)
-    const int id = __builtin_amdgcn_readlane(ids, p - ids_at);
-    return (unsigned)id < (unsigned)a.num_pages ? id : 0;
-  };
-  vec8_t<T> k0[DK / 32], k1[DK / 32], v[DV / 16];
-  auto load_keys = [&](int cb, int id) {
-    const T* kp = kbase + (paged ? (long)id * 64 + (cb & 63) : (long)b * a.ctx_cap + cb) * krow;
-    const T* k0p = kp + chunk_key_of_row(0, n16) * krow;
-    const T* k1p = kp + chunk_key_of_row(1, n16) * krow;
+    const float c = a.scale * kLog2e;
+
+    // chunk i of this wavefront covers keys 64 p0 + 32 (w + W i) ..; 64 page ids at a time sit in the lanes
+    int ids_at = p0, ids = 0;
+    if (paged && p0 + lane < p1) ids = table[p0 + lane];
+    auto page_of = [&](int cb) -> int {
+      const int p = cb >> 6;
+      if (p - ids_at >= 64) {
+        ids_at = p;
+        ids = p + lane < p1 ? table[p + lane] : 0;
+      }
+      // an id outside the pool would fault: read page 0 instead (the caller's table is wrong)
+      const int id = __builtin_amdgcn_readlane(ids, p - ids_at);
+      return (unsigned)id < (unsigned)a.num_pages ? id : 0;
+    };
+    vec8_t<T> k0[DK / 32], k1[DK / 32], v[DV / 16];
+    auto load_keys = [&](int cb, int id) {
+      const T* kp = kbase + (paged ? (long)id * 64 + (cb & 63) : (long)b * a.ctx_cap + cb) * krow;
+      const T* k0p = kp + chunk_key_of_row(0, n16) * krow;
+      const T* k1p = kp + chunk_key_of_row(1, n16) * krow;
 #pragma unroll
-    for (int kk = 0; kk < DK / 32; ++kk) { k0[kk] = load8(k0p + 32 * kk); k1[kk] = load8(k1p + 32 * kk); }
-  };
-  auto load_values = [&](int cb, int id) {
-    const T* vp = vbase + ((long)(paged ? id : b) * a.hkv + h) * DV * vrow + (paged ? (cb & 63) : cb) + (long)n16 * vrow + 8 * g;
+      for (int kk = 0; kk < DK / 32; ++kk) { k0[kk] = load8(k0p + 32 * kk); k1[kk] = load8(k1p + 32 * kk); }
+    };
+    auto load_values = [&](int cb, int id) {
+      const T* vp = vbase + ((long)(paged ? id : b) * a.hkv + h) * DV * vrow + (paged ? (cb & 63) : cb) + (long)n16 * vrow + 8 * g;
 #pragma unroll
-    for (int t = 0; t < DV / 16; ++t) v[t] = load8(vp + 16 * t * vrow);
-  };
-  // the next chunk's keys are requested as soon as the scores have used this one's, its values after the second
-  // product: one set of registers, and loads of this wavefront are always in flight
-  const int end = min(p1 * 64, sp.n);
-  int cb = p0 * 64 + 32 * w;
-  if (cb < end) {
+      for (int t = 0; t < DV / 16; ++t) v[t] = load8(vp + 16 * t * vrow);
+    };
+    // the next chunk's keys are requested as soon as the scores have used this one's, its values after the second
+    // product: one set of registers, and loads of this wavefront are always in flight
+    const int end = min(p1 * 64, sp.n);
+    int cb = p0 * 64 + 32 * w;
+    if (cb >= end) return;
     int id = paged ? page_of(cb) : 0;
     load_keys(cb, id);
     load_values(cb, id);
@@ -275,12 +301,34 @@ dense_decode_kernel(const DenseDecodeArgs a) {
       const int next = cb + 32 * W;
       if (next < end) {
         id = paged ? page_of(next) : 0;
-        load_keys(next, id);
+        if (!kOdd) load_keys(next, id);
       }
-      dense_values<T, DK, DV, NT>(st, v, s, cb, sp.lo, sp.n, c, g);
+      dense_values<kOdd, T, DK, DV, NT>(st, v, s, cb, sp.lo, sp.n, c, g, finite);
       if (next >= end) break;
+      if (kOdd) load_keys(next, id);         // it has no registers to spare
       load_values(next, id);
       cb = next;
+    }
+  };
+  stream(std::false_type(), true, lane);
+  if constexpr (sizeof(T) == 2) {
+    // once something is infinite or no number, the sums stay so: only then the unit is read again
+    unsigned top = 0;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int t = 0; t < DV / 16; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(st[j].o[t][i]) << 1);
+    if (__any(top >= 0xff000000u)) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) dec_reset(st[j]);
+#pragma unroll 1
+      for (int pass = 0; pass < 2; ++pass) {
+        int again = lane;
+        asm volatile("" : "+v"(again));      // what follows from it is worked out anew, not kept in registers all along
+        stream(std::true_type(), pass == 0, again);
+      }
     }
   }
 
@@ -374,7 +422,10 @@ dense_decode_join_kernel(const DenseDecodeArgs a, int rows_per_slot, int blocks)
     float mx = m;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      if (u + k * kGroups >= count) um[k] = kNegInf;       // the last unit once more
+      if (u + k * kGroups >= count) {                      // the last unit once more: infinity times a weight of 0 is NaN
+        um[k] = kNegInf;
+        uo[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      }
       mx = fmaxf(mx, um[k]);
     }
     const float ref = mx == kNegInf ? 0.f : mx;

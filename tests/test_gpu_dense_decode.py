@@ -420,3 +420,63 @@ def test_results_that_overlap_the_operands_are_refused():
     want, _ = check(q, c, ks, vs)
     got, _ = check(q, c, ks, vs, out=out_at(2 * n), lse=lse_at(3 * n))
     assert torch.equal(got, want) and torch.equal(dense_decode_step(q, c, out=out_at(0)), want)
+
+
+@pytest.mark.parametrize("paged", [True, False])
+@pytest.mark.parametrize("cap", [192, 2048])                      # one launch, and the split schedule
+@pytest.mark.parametrize("dtype,group,dk,dv", [(torch.bfloat16, 4, 64, 64), (torch.float16, 4, 64, 64), (torch.float32, 4, 64, 64),
+                                               (torch.bfloat16, 16, 128, 128), (torch.float16, 20, 32, 32),
+                                               (torch.bfloat16, 64, 192, 128), (torch.float16, 40, 128, 128)])
+def test_infinities_among_the_visible_values_come_through(paged, cap, dtype, group, dk, dv):
+    """a value of infinity makes its channel infinite for the heads that read it, one of each sign no number; every other
+    channel and the log-sum-exp keep their bits"""
+    from nsa_amd.decode import dense_decode_step
+    lens = [1, 190, cap, 64, 33]
+    c, ks, vs = make_cache(paged, lens, cap, 2, dk, dv, dtype, seed=150)
+    q = randn(len(lens), 2 * group, dk, seed=151, dtype=dtype).to(DEV)
+    want, want_lse = dense_decode_step(q, c, return_lse=True)
+    expect = want.clone()
+
+    def put(b, h, chan, key, x):
+        if paged:
+            c.v_pool_t[c.block_table[b, key // 64].long(), h, chan, key % 64] = x
+        else:
+            c.vt[b, h, chan, key] = x
+
+    for b, h, chan, puts in ((0, 0, 3, [(0, math.inf)]), (0, 1, dv - 1, [(0, -math.inf)]), (1, 0, 0, [(0, math.inf)]),
+                             (1, 0, 17, [(189, -math.inf), (3, -math.inf)]), (1, 1, 5, [(70, math.inf), (71, -math.inf)]),
+                             (2, 1, 9, [(cap - 1, math.inf)]), (2, 1, 10, [(5, -math.inf), (cap - 40, math.inf)]),
+                             (2, 0, 11, [(31, math.nan), (32, math.inf)]), (4, 0, 20, [(32, -math.inf)])):
+        for key, x in puts:
+            put(b, h, chan, key, x)
+        expect[b, h * group:(h + 1) * group, chan] = sum(x for _, x in puts)
+    out, lse = dense_decode_step(q, c, return_lse=True)
+    assert torch.equal(out.isnan(), expect.isnan()) and torch.equal(out.nan_to_num(0.5), expect.nan_to_num(0.5))
+    assert torch.equal(lse, want_lse)
+    # before a window they do not matter
+    out, lse = dense_decode_step(q, c, sliding_window=1, return_lse=True)
+    for b, n in enumerate(lens):
+        hidden = [x for x in ((0, 0, 3), (0, 1, dv - 1)) if b == 0] + [x for x in ((2, 1, 9),) if b == 2] + \
+            [x for x in ((1, 0, 17),) if b == 1] + [x for x in ((4, 0, 20),) if b == 4]
+        finite = torch.ones(2 * group, dv, dtype=torch.bool, device=DEV)
+        for _, h, chan in hidden:
+            finite[h * group:(h + 1) * group, chan] = False
+        assert torch.equal(out[b].isfinite(), finite), b
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_an_infinity_far_below_the_maximum_counts(dtype):
+    """weights of 2^-60 beside the largest: 0 in float16, but not the formula's"""
+    from nsa_amd.decode import dense_decode_step
+    lens = [200]
+    c, ks, vs = make_cache(True, lens, 256, 1, 64, 64, dtype, seed=160)
+    c.k_pool.zero_()
+    c.k_pool[c.block_table[0, 1].long(), 0, 0, 0] = 1.0                          # key 64: 60 ln 2 above all others
+    c.v_pool_t[c.block_table[0, 2].long(), 0, 7, 1] = -math.inf
+    q = torch.zeros(1, 4, 64, dtype=dtype, device=DEV)
+    q[:, :, 0] = 1.0
+    out = dense_decode_step(q, c, scale=60 * math.log(2))
+    assert (out[0, :, 7] == -math.inf).all()
+    rest = [i for i in range(64) if i != 7]
+    v = vs[0][64, 0, rest].double().to(DEV)                                      # all of the weight but 200 * 2^-60
+    assert ((out[0, :, rest].double() - v).abs() <= 2.0 ** -21 * v.abs() + 2.0 ** -50).all()
