@@ -460,7 +460,8 @@ int nsa_decode_step_split_static(const void* q, const void* k_cache, const void*
  *   q [batch][hq][dk]   out [batch][hq][dv]   lse (optional) float [batch][hq]: natural-log log-sum-exp of the scaled scores
  * A sequence with ctx_lens[b] <= 0 yields out = 0 and lse = -inf; a length beyond the capacity counts as the capacity.
  * What the cache holds behind a sequence's last token, or before its window, does not matter (not even NaN).  A table
- * entry outside the pool is read as page 0.  Any GQA group size; (dk, dv) in (32,32), (64,64), (128,128), (192,128).
+ * entry outside the pool is read as page 0.  Infinities and NaN in visible rows come out as the formula gives them; the
+ * sums sum exp(s - m) v are held in fp32 before the division, so they have to fit it.  Any GQA group size; (dk, dv) in (32,32), (64,64), (128,128), (192,128).
  * The cached tokens of all sequences are cut into equal pieces on the device, from ctx_lens, so the grid and the
  * workspace depend on the arguments alone and a captured call stays right while the sequences grow.  The result of a
  * sequence depends on where it is cut, hence to rounding on the other lengths of the batch; equal calls give equal bits.

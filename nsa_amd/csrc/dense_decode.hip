@@ -86,10 +86,12 @@ __device__ __forceinline__ int dense_unit_pages(const DenseDecodeArgs& a) {
   return C;
 }
 
-// How far below the running maximum the reference of the exponentials lies.  float16 ends at 2^-24: with probabilities of up
-// to 2^(7 + 8) instead of 1 it keeps what lies 2^-31 below the maximum, which thousands of such keys add up to (one key
-// that takes nearly all the weight, 1000 others at 2^-26 each: 1/8 of their sum was lost without).
-template <typename T> constexpr float kDenseBelow = 0.0f;
+// How far below the running maximum the reference of the exponentials is put.  In 32 bits and bfloat16 it goes 2^8 above, by
+// which the maximum may then grow before the sums are rescaled, so that no probability passes 1 and the sums end where those
+// of the formula do (with probabilities of up to 2^8 values of 2^119 overflowed).  float16 ends at 2^-24 and its values at
+// 2^16: with probabilities of up to 2^(7 + 8) it keeps what lies 2^-31 below the maximum, which thousands of such keys add up
+// to (one key that takes nearly all the weight, 1000 others at 2^-26 each: 1/8 of their sum was lost without).
+template <typename T> constexpr float kDenseBelow = -kMaxSlackLog2;
 template <> constexpr float kDenseBelow<f16_t> = 7.0f;
 
 // A 16-bit value that is no number or infinite, by its bits (the library is compiled with the promise that no NaN occurs).
@@ -151,7 +153,7 @@ __device__ __forceinline__ void dense_values(DecState<T, DK, DV> (&st)[NT], vec8
       mx = fmaxf(mx, whole || (key >= lo && key < n) ? x : kNegInf);
     }
     // The reference of the exponentials follows the maximum only when that has grown by more than 2^8 (the first chunk, and
-    // hardly ever again): probabilities stay below 2^8 (float16: 2^15), and the sums are not rescaled at every chunk.
+    // hardly ever again): probabilities stay within 1 (float16: 2^15), and the sums are not rescaled at every chunk.
     mx = colgroup_max(mx);
     constexpr float below = kDenseBelow<T>;
     if (__any(mx > st[j].m + (kMaxSlackLog2 + below))) {

@@ -480,3 +480,27 @@ def test_an_infinity_far_below_the_maximum_counts(dtype):
     rest = [i for i in range(64) if i != 7]
     v = vs[0][64, 0, rest].double().to(DEV)                                      # all of the weight but 200 * 2^-60
     assert ((out[0, :, rest].double() - v).abs() <= 2.0 ** -21 * v.abs() + 2.0 ** -50).all()
+
+
+@pytest.mark.parametrize("lens,big", [([300, 1, 40], 119), ([2048] * 63 + [2000], 116)])   # one launch; units of 4 pages and more
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_values_near_the_end_of_the_range_do_not_overflow(lens, big, dtype):
+    """Values of 2^big under weights that rise by 2^7.9 after a wavefront's first keys: sum exp(s - m) |v| stays below
+    n 2^big < 2^128, so the sums have to, whatever the reference of the exponentials."""
+    from nsa_amd.decode import NSADecodeCache
+    c = NSADecodeCache(len(lens), max(lens), 1, 64, 64, dtype=dtype, device=DEV)
+    key = torch.arange(max(lens))
+    high = key % 256 >= 128 if len(lens) > 3 else key >= 256
+    k = torch.zeros(max(lens), 1, 64)
+    k[high, 0, 0] = 5.46875                                                  # 7.89 ln 2
+    v = torch.full((max(lens), 1, 64), 2.0 ** big)
+    v[:, :, ::2] *= -1
+    v[:, :, 5] = 1.0
+    ks, vs = [k[:n].to(dtype) for n in lens], [v[:n].to(dtype) for n in lens]
+    for b, n in enumerate(lens):
+        c.k[b, :n] = ks[b].to(DEV)
+        c.vt[b, :, :, :n] = vs[b].permute(1, 2, 0).to(DEV)
+    c.ctx_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+    q = torch.zeros(len(lens), 4, 64, dtype=dtype, device=DEV)
+    q[:, :, 0] = 1.0
+    check(q, c, ks, vs, scale=1.0)
