@@ -118,10 +118,12 @@ class NSAPagedDecodeCache:
     (rejected drafts), compact() moves the pages in use together.  Full pages are shared by reference count; the partly
     filled last page of a sequence is always its own, so append() never writes into a shared page.
 
-    Page bookkeeping (free list, lengths, counts) lives on the host, so no call here waits for the GPU.  One cache is
-    used by one thread and one stream at a time."""
+    Page bookkeeping (free list, lengths, counts) lives on the host, so no call here waits for the GPU.  If the device half
+    of a move fails (a launch error), the host's books no longer fit the device's: the call raises, and so does every later
+    one that would change the cache.  Calls that change a cache are made by one thread and on one stream at a time."""
 
     PAGE = 64
+    _lost = False                                        # whether a move's device half failed
     _BOOKS = ("_table", "_lens", "_held", "_refs")       # arrays that the library shares
 
     def __init__(self, batch, num_pages, max_ctx, hkv, dk, dv, block=32, stride=16, dtype=torch.bfloat16,
@@ -166,7 +168,18 @@ class NSAPagedDecodeCache:
         for name in self._BOOKS:
             setattr(self, name, (C.c_int32 * len(state[name]))(*state[name]))
 
+    def _check_lost(self):
+        if self._lost:
+            raise RuntimeError("an earlier move of this cache failed on the device, whose page table no longer fits the "
+                               "host's: build a new cache")
+
+    def _device_half(self, name, *args):
+        self._lost = True
+        _lib.check(getattr(_lib.load(), name)(*args), name)
+        self._lost = False
+
     def _books(self):
+        self._check_lost()
         return (self._table, self._lens, self._held, self._refs, self._free.ids, C.byref(self._free.n), self.batch,
                 self.max_pages, self.num_pages)
 
@@ -292,12 +305,10 @@ class NSAPagedDecodeCache:
         code = _dtype_code(self.k_pool)
         moves, n_moves = self._plan(slots, parents, lengths)
         self._shares = True
-        rc = _lib.load().nsa_paged_cache_move(
-            self.k_pool.data_ptr(), self.v_pool_t.data_ptr(), self.block_table.data_ptr(), self.ck.data_ptr(),
-            self.cvt.data_ptr(), self.ctx_lens.data_ptr(), moves, n_moves, self.batch, self.max_pages, self.num_pages,
-            self.hkv, self.dk, self.dv, self.nc_cap, self.block, self.stride, code, _raw_stream(device))
-        if rc:
-            _lib.check(rc, "nsa_paged_cache_move")
+        self._device_half(
+            "nsa_paged_cache_move", self.k_pool.data_ptr(), self.v_pool_t.data_ptr(), self.block_table.data_ptr(),
+            self.ck.data_ptr(), self.cvt.data_ptr(), self.ctx_lens.data_ptr(), moves, n_moves, self.batch, self.max_pages,
+            self.num_pages, self.hkv, self.dk, self.dv, self.nc_cap, self.block, self.stride, code, _raw_stream(device))
 
     @staticmethod
     def _ids(slots):
@@ -356,15 +367,15 @@ class NSAPagedDecodeCache:
         pairs, n_pairs, used = (C.c_int32 * (2 * self.num_pages))(), C.c_int32(), C.c_int32()
         rc = lib.nsa_paged_cache_compact_plan(*self._books(), pairs, C.byref(n_pairs), C.byref(used))
         _lib.check(rc, "nsa_paged_cache_compact_plan")
-        rc = lib.nsa_paged_cache_compact_move(
-            self.k_pool.data_ptr(), self.v_pool_t.data_ptr(), self.block_table.data_ptr(), pairs, n_pairs.value, self.batch,
-            self.max_pages, self.num_pages, self.hkv, self.dk, self.dv, code, _raw_stream(device))
-        _lib.check(rc, "nsa_paged_cache_compact_move")
+        self._device_half(
+            "nsa_paged_cache_compact_move", self.k_pool.data_ptr(), self.v_pool_t.data_ptr(), self.block_table.data_ptr(), pairs,
+            n_pairs.value, self.batch, self.max_pages, self.num_pages, self.hkv, self.dk, self.dv, code, _raw_stream(device))
         return used.value
 
     def reserve_next(self):
         """Host half of append(): makes sure every sequence owns the page of its next token and
         publishes new table entries.  Separate so that the device half can live in a captured graph."""
+        self._check_lost()
         lens = self._lens[:]
         fresh = [b for b, n in enumerate(lens) if n % self.PAGE == 0]
         if len(fresh) > len(self._free):

@@ -402,3 +402,37 @@ def test_sampling_from_a_prompt_with_pictures():
                 shared.compact()
     check_books(shared)
     assert shared.free_pages > apart.free_pages
+
+
+class FailingLibrary:
+    """The library with one function that fails before it does anything."""
+
+    def __init__(self, lib, name):
+        self.lib, self.name = lib, name
+
+    def __getattr__(self, name):
+        return (lambda *a: -4) if name == self.name else getattr(self.lib, name)
+
+
+@pytest.mark.parametrize("name", ["nsa_paged_cache_move", "nsa_paged_cache_compact_move"])
+def test_a_cache_whose_device_half_failed_takes_no_more_calls(name, monkeypatch):
+    """the page table of the host is then ahead of the device's, so nothing may be built on it; reading goes on"""
+    from nsa_amd import _lib
+    from nsa_amd.decode import dense_decode_step
+    c = filled([100, 130, 64], 256)
+    c.truncate(0, 30)
+    k, v = randn(3, 2, 64, seed=1, dtype=torch.bfloat16).to(DEV), randn(3, 2, 64, seed=2, dtype=torch.bfloat16).to(DEV)
+    q = randn(3, 4, 64, seed=3, dtype=torch.bfloat16).to(DEV)
+    want, tables = dense_decode_step(q, c), [t.clone() for t in (c.block_table, c.ctx_lens, c.k_pool, c.v_pool_t, c.ck, c.cvt)]
+    lib = _lib.load()
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "load", lambda: FailingLibrary(lib, name))
+        with pytest.raises(RuntimeError, match="failed"):
+            c.compact() if "compact" in name else c.reorder([1, 2, 0])
+    for call in (lambda: c.fork(0, 1), lambda: c.reorder([0, 0, 1]), lambda: c.truncate(1, 5), lambda: c.release(1),
+                 lambda: c.compact(), lambda: c.append(k, v), lambda: c.reserve_next(),
+                 lambda: c.fill(k.expand(70, -1, -1, -1)[:, 0].contiguous(), v.expand(70, -1, -1, -1)[:, 0].contiguous(), seq=2)):
+        with pytest.raises(RuntimeError, match="build a new"):
+            call()
+    assert same(tables, [c.block_table, c.ctx_lens, c.k_pool, c.v_pool_t, c.ck, c.cvt])
+    assert torch.equal(dense_decode_step(q, c), want)
