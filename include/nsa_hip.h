@@ -47,6 +47,7 @@ enum {
   NSA_ERR_LAUNCH = -4       /* HIP reported a launch failure */
 };
 enum { NSA_GATE_IDENTITY = 0, NSA_GATE_SIGMOID = 1 };
+enum { NSA_POSITIONS_I64 = 256 };            /* added to `axes` of nsa_qkv_rope_axes */
 
 int nsa_version(void);
 const char* nsa_last_error_string(void);
@@ -201,13 +202,13 @@ int nsa_qkv_rope(void* packed, void* q, void* k, void* v, void* gates, const flo
 
 /* nsa_qkv_rope with positions on several axes (time, height and width of a picture's or film's tokens): pair i of the
  * rotary channels turns by positions[pair_axis[i]][t] * inv_freq[i].
- *   positions int32 [axes][total], axes 1..4;  pair_axis int32 [rope_dim / 2], a HOST pointer, read during the call
+ *   positions int32 [axes][total], axes 1..4, or int64 with axes + NSA_POSITIONS_I64;  pair_axis int32 [rope_dim / 2], a HOST pointer, read during the call
  * The angle is formed in 64 bits, so that far positions keep their phase.  inv_freq is required; the other arguments are
  * those of nsa_qkv_rope.  pack = 1 also clears the columns of a row behind the last of the four
  * ranges, which must not overlap then.  The reference's
  * caller rotates before NSAAttention.forward (nsa/nsa.py:83-135); it has no kernel for it. */
 int nsa_qkv_rope_axes(void* packed, void* q, void* k, void* v, void* gates, const float* inv_freq,
-                      const int32_t* positions, int axes, const int32_t* pair_axis, int64_t total, int ld, int q_off,
+                      const void* positions, int axes, const int32_t* pair_axis, int64_t total, int ld, int q_off,
                       int k_off, int v_off, int g_off, int hq, int hkv, int dk, int dv, int rope_off, int rope_dim,
                       int interleaved, int pack, int dtype, nsa_stream_t stream);
 

@@ -324,9 +324,11 @@ int nsa_qkv_rope(void* packed, void* q, void* k, void* v, void* gates, const flo
 }
 
 int nsa_qkv_rope_axes(void* packed, void* q, void* k, void* v, void* gates, const float* inv_freq,
-                      const int32_t* positions, int axes, const int32_t* pair_axis, int64_t total, int ld, int q_off,
+                      const void* positions, int axes, const int32_t* pair_axis, int64_t total, int ld, int q_off,
                       int k_off, int v_off, int g_off, int hq, int hkv, int dk, int dv, int rope_off, int rope_dim,
                       int interleaved, int pack, int dtype, nsa_stream_t stream) {
+  const bool wide = axes > 0 && (axes & NSA_POSITIONS_I64);
+  if (wide) axes -= NSA_POSITIONS_I64;
   if (!packed || !q || !k || !v || !inv_freq || !positions || !pair_axis)
     return fail(NSA_ERR_INVALID, "qkv_rope_axes: null pointer");
   if (!dtype_ok(dtype)) return fail(NSA_ERR_INVALID, "qkv_rope_axes: bad dtype");
@@ -343,6 +345,8 @@ int nsa_qkv_rope_axes(void* packed, void* q, void* k, void* v, void* gates, cons
                                  "(length a multiple of 16, or of 8 when interleaved)");
   if (rope_dim > 256) return fail(NSA_ERR_UNSUPPORTED, "qkv_rope_axes: more than 256 rotary channels");
   if (axes < 1 || axes > 4) return fail(NSA_ERR_INVALID, "qkv_rope_axes: 1 to 4 axes");
+  if (reinterpret_cast<uintptr_t>(positions) % (wide ? 8 : 4) != 0)
+    return fail(NSA_ERR_INVALID, "qkv_rope_axes: positions must be aligned to their type");
   nsa::RopeAxesArgs a{};
   for (int i = 0; i < rope_dim / 2; ++i) {
     if (pair_axis[i] < 0 || pair_axis[i] >= axes) return fail(NSA_ERR_INVALID, "qkv_rope_axes: pair %d names axis %d of %d", i, pair_axis[i], axes);
@@ -350,7 +354,9 @@ int nsa_qkv_rope_axes(void* packed, void* q, void* k, void* v, void* gates, cons
   }
   if (!aligned16(packed) || !aligned16(q) || !aligned16(k) || !aligned16(v))
     return fail(NSA_ERR_INVALID, "qkv_rope_axes: pointers must be 16-byte aligned");
-  a.base = nsa::QkvRopeArgs{packed, q, k, v, gates, inv_freq, positions, nullptr, 0, (long)total, ld, q_off, k_off, v_off,
+  a.positions = positions;
+  a.wide = wide;
+  a.base = nsa::QkvRopeArgs{packed, q, k, v, gates, inv_freq, nullptr, nullptr, 0, (long)total, ld, q_off, k_off, v_off,
                             g_off, hq, hkv, dk, dv, rope_off, rope_dim, interleaved ? 1 : 0, pack ? 1 : 0, dtype};
   const int64_t at[4][2] = {{q_off, nq}, {k_off, nk}, {v_off, nv}, {g_off, gates ? ng : 0}};
   for (int i = 0; i < 4 && pack; ++i)

@@ -202,7 +202,8 @@ struct QkvRopeArgs {
 int launch_qkv_rope(const QkvRopeArgs& a, hipStream_t st);
 // The same with positions [axes][total]: pair i turns by positions[axis of pair i]; two bits per pair name the axis.
 struct RopeAxesArgs {
-  QkvRopeArgs base;
+  QkvRopeArgs base;                                        // its positions are not used
+  const void* positions; bool wide;                        // int32, wide: int64
   unsigned pair_axis[8];
   int pad_off;                                             // pack: columns [pad_off, ld) of a row are cleared
   bool vector_gates; int pieces, cols, side;                                  // filled in by the launch: pieces per row, per workgroup, rows beside each other

@@ -19,7 +19,8 @@ namespace nsa {
 // neighbouring columns of the same rows: 327 us against 386 with neighbouring rows.
 template <typename T> constexpr int kRopeRows = sizeof(T) == 2 ? 2 : 1;
 
-template <typename T, bool PACK, int U>
+// P: type of the positions.  A choice between the two inside the kernel cost 5 % (32768 rows: 328 -> 344 us).
+template <typename T, typename P, bool PACK, int U>
 __global__ void __launch_bounds__(256)
 rope_axes_kernel(const RopeAxesArgs a) {
   extern __shared__ float2 turn[];                       // [row of the workgroup][pair]: cosine, sine
@@ -84,7 +85,7 @@ rope_axes_kernel(const RopeAxesArgs a) {
       const long t = w0 + k;
       if (t < r.total) {
         const int axis = (a.pair_axis[pair >> 4] >> (2 * (pair & 15))) & 3;
-        const double turns = (double)r.positions[axis * r.total + t] * ((double)r.inv_freq[pair] * 0.15915494309189535);
+        const double turns = (double)reinterpret_cast<const P*>(a.positions)[axis * r.total + t] * ((double)r.inv_freq[pair] * 0.15915494309189535);
         float s, c;
         sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
         turn[i] = make_float2(c, PACK ? -s : s);
@@ -144,24 +145,30 @@ rope_axes_kernel(const RopeAxesArgs a) {
   }
 }
 
-template <typename T, bool PACK, int U>
+template <typename T, typename P, bool PACK, int U>
 static int rope_axes_u(const RopeAxesArgs& a, hipStream_t st) {
   const long blocks = (a.base.total + U * a.side - 1) / (U * a.side);
   const long slices = (a.pieces + a.cols - 1) / a.cols;
   if (blocks * slices > 0x7fffffffL) return -2;
   const unsigned threads = (unsigned)(a.cols * a.side + 63) / 64 * 64;
   const size_t smem = (size_t)U * a.side * (a.base.rope_dim / 2) * sizeof(float2);
-  hipLaunchKernelGGL((rope_axes_kernel<T, PACK, U>), dim3((unsigned)(blocks * slices)), dim3(threads), smem, st, a);
+  hipLaunchKernelGGL((rope_axes_kernel<T, P, PACK, U>), dim3((unsigned)(blocks * slices)), dim3(threads), smem, st, a);
   return 0;
 }
 
-template <typename T>
+template <typename T, typename P>
 static int rope_axes_t(const RopeAxesArgs& a, hipStream_t st) {
   // few rows: one per thread, over twice the workgroups (1000 rows of 4 / 1 heads of 64: 4.8 against 6.2 us)
   constexpr int U = kRopeRows<T>;
   const bool large = a.base.total * (long)a.pieces >= 1L << 18;
-  if (a.base.pack) return large ? rope_axes_u<T, true, U>(a, st) : rope_axes_u<T, true, 1>(a, st);
-  return large ? rope_axes_u<T, false, U>(a, st) : rope_axes_u<T, false, 1>(a, st);
+  if (a.base.pack) return large ? rope_axes_u<T, P, true, U>(a, st) : rope_axes_u<T, P, true, 1>(a, st);
+  return large ? rope_axes_u<T, P, false, U>(a, st) : rope_axes_u<T, P, false, 1>(a, st);
+}
+
+template <typename P>
+static int rope_axes_p(const RopeAxesArgs& a, hipStream_t st) {
+  if (a.base.dtype == 2) return rope_axes_t<f16_t, P>(a, st);
+  return a.base.dtype == 0 ? rope_axes_t<bf16_t, P>(a, st) : rope_axes_t<float, P>(a, st);
 }
 
 int launch_rope_axes(RopeAxesArgs a, hipStream_t st) {
@@ -177,8 +184,7 @@ int launch_rope_axes(RopeAxesArgs a, hipStream_t st) {
   a.side = 256 / a.cols;
   // short rows whose heads have many pairs keep to fewer rows: at most 32 KB of sines
   while (a.side > 1 && 2 * a.side * (r.rope_dim / 2) * sizeof(float2) > 32768) --a.side;
-  if (r.dtype == 2) return rope_axes_t<f16_t>(a, st);
-  return r.dtype == 0 ? rope_axes_t<bf16_t>(a, st) : rope_axes_t<float>(a, st);
+  return a.wide ? rope_axes_p<int64_t>(a, st) : rope_axes_p<int32_t>(a, st);
 }
 
 }  // namespace nsa

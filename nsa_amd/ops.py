@@ -748,7 +748,9 @@ def _qkv_rope_axes(packed, q, k, v, gates, offsets, inv_freq, positions, rope_of
         return
     dev = packed.device
     inv_freq = inv_freq.to(device=dev, dtype=torch.float32).contiguous()
-    positions = positions.to(device=dev, dtype=torch.int32).contiguous()
+    # int64 and int32 as they are; what int32 does not hold goes as int64
+    wide = positions.dtype in (torch.int64, torch.uint32, torch.uint64)
+    positions = positions.to(device=dev, dtype=torch.int64 if wide else torch.int32).contiguous()
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return _qkv_rope_axes(packed, q, k, v, gates, offsets, inv_freq, positions, rope_off, rope_dim, interleaved,
@@ -756,8 +758,9 @@ def _qkv_rope_axes(packed, q, k, v, gates, offsets, inv_freq, positions, rope_of
     q_off, k_off, v_off, g_off = offsets
     rc = _lib.load().nsa_qkv_rope_axes(
         packed.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), None if gates is None else gates.data_ptr(),
-        inv_freq.data_ptr(), positions.data_ptr(), positions.shape[0], axis_of, total, packed.shape[1], q_off, k_off,
-        v_off, g_off, hq, hkv, dk, dv, rope_off, rope_dim, bool(interleaved), pack, _dtype_code(packed), _raw_stream(dev))
+        inv_freq.data_ptr(), positions.data_ptr(), positions.shape[0] + wide * _lib.POSITIONS_I64, axis_of, total,
+        packed.shape[1], q_off, k_off, v_off, g_off, hq, hkv, dk, dv, rope_off, rope_dim, bool(interleaved), pack,
+        _dtype_code(packed), _raw_stream(dev))
     if rc:
         _lib.check(rc, "nsa_qkv_rope_axes")
 
@@ -769,7 +772,7 @@ def qkv_rope_split(packed, hq, hkv, dk, dv, offsets, inv_freq=None, positions=No
     [total,hkv,dv], gates [total,hq,3] or None; channels [rope_off, rope_off+rope_dim) of every q and
     k head are rotated by position * inv_freq[i] (positions int32 [total], or the offset inside the
     sequence from cu_seqlens).
-    pair_axis (one axis number per pair of rotary channels): positions are whole numbers [axes, total] on up to four axes,
+    pair_axis (one axis number per pair of rotary channels): positions are whole numbers (to 64 bits) [axes, total] on up to four axes,
     e.g. time, height and width, and pair i turns by positions[pair_axis[i]] * inv_freq[i], the angle formed in 64 bits;
     cu_seqlens is not read."""
     _need_cuda(packed)

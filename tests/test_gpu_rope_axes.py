@@ -384,3 +384,40 @@ def test_layer_decode_step_takes_the_new_tokens_positions():
     # the decode step and the prefill row round probabilities, branches and the projection separately
     u = torch.finfo(torch.bfloat16).eps / 2
     assert float((steps[0] - rows).abs().float().mean()) <= 8 * u * float(rows.abs().float().mean())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_positions_beyond_32_bits_keep_all_of_theirs(dtype):
+    """int64 positions, forward and backward.  The angle is a product of two rounded 64-bit numbers there, in the reference
+    too, each off by 2^-52 of itself at most: the bound has |angle| 2^-51 more."""
+    from nsa_amd import ops
+    from nsa_amd.autograd import QkvRopeFn
+    hq, hkv, dk, dv, dim = 4, 2, 64, 64, 64
+    at, ld = layout(hq, hkv, dk, dv)
+    pos = torch.tensor([[2 ** 31, -2 ** 31 - 1, 2 ** 32 + 5, 7, -2 ** 34 - 99, 3], [0, 2 ** 33 + 2 ** 20 + 1, -1, 2 ** 31 + 12345,
+                        2 ** 35 + 17, -2 ** 31]])
+    pair_axis, inv = [i % 2 for i in range(32)], freqs(32)
+    far = (pos.double().abs().amax(0) * 2.0 ** -51)[:, None, None]
+    kw = dict(inv_freq=inv, positions=pos.to(DEV), rope_off=0, rope_dim=dim, pair_axis=pair_axis)
+
+    def check(got, x, sign):
+        ref, slack = rotated(x, pos, pair_axis, inv, 0, False, sign)
+        x = x.double().abs()
+        close(got, ref, slack + (x + x.roll(32, -1)) * far)
+
+    packed = randn(6, ld, seed=17, dtype=dtype)
+    q, k, v, gates = ops.qkv_rope_split(packed.to(DEV), hq, hkv, dk, dv, at, **kw)
+    check(q, packed[:, :at[1]].reshape(6, hq, dk), 1.0)
+    check(k, packed[:, at[1]:at[2]].reshape(6, hkv, dk), 1.0)
+    d = ops.qkv_rope_pack(q, k, v, gates, ld, at, **kw).cpu()
+    check(d[:, :at[1]].reshape(6, hq, dk), q.cpu(), -1.0)
+    x = packed.to(DEV).requires_grad_()
+    outs = QkvRopeFn.apply(x, hq, hkv, dk, dv, at, inv, kw["positions"], None, 0, dim, False, True, pair_axis)
+    assert torch.equal(outs[0], q)
+    torch.autograd.backward(outs, [t.detach() for t in outs])
+    assert torch.equal(x.grad.cpu(), d)
+    # and those that fit are the same in either type
+    near = torch.tensor([[2 ** 31 - 1, -2 ** 31, 5, 0, -9, 77]] * 2)
+    both = [ops.qkv_rope_split(packed.to(DEV), hq, hkv, dk, dv, at, **dict(kw, positions=near.to(DEV, t)))[0]
+            for t in (torch.int64, torch.int32)]
+    assert torch.equal(*both)

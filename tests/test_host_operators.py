@@ -564,3 +564,19 @@ def test_dense_decode_refuses_results_on_top_of_its_operands(lib):
     assert refused(table=None, cap=64 * width, max_pages=0, num_pages=0, out=last)
     # its type decides how far an operand reaches
     assert refused(dtype=1, ws_bytes=1 << 31, out=at["q"] + B * hq * dk * 2)
+
+
+def test_rope_axes_takes_the_position_type_with_the_axes(lib):
+    """refused before a launch: no axes beside the flag, five of them, an axis they do not have, 8-byte positions off by 4"""
+    buf = (ctypes.c_char * 4096)()
+    p = ctypes.addressof(buf) + (-ctypes.addressof(buf)) % 16
+    pairs = (ctypes.c_int32 * 128)(0, 1, 2)
+
+    def call(axes, pos=p):
+        return lib.nsa_qkv_rope_axes(p, p, p, p, p, p, pos, axes, pairs, 4, 416, 0, 256, 320, 384, 4, 1, 64, 64, 0, 32, 0, 0,
+                                     0, None)
+
+    for axes in (256, 256 + 5, 256 + 2, 512 + 3, 3 - 256):
+        assert call(axes) == -1
+    assert call(256 + 3, p + 4) == -1 and b"aligned to their type" in lib.nsa_last_error_string()
+    assert call(3, p + 2) == -1 and b"aligned to their type" in lib.nsa_last_error_string()
