@@ -504,3 +504,58 @@ def test_values_near_the_end_of_the_range_do_not_overflow(lens, big, dtype):
     q = torch.zeros(len(lens), 4, 64, dtype=dtype, device=DEV)
     q[:, :, 0] = 1.0
     check(q, c, ks, vs, scale=1.0)
+
+
+# ---- float16 at the bound its reference of 2^7 below the maximum allows: l is at least 2^7 where a probability is off by 2^-25
+# at most (float16's last step), so the term is 2^-32 n max |v| instead of plain()'s 2^-25 n max |v|
+
+def check_float16(q, c, ks, vs, window=0, scale=None):
+    from nsa_amd.decode import dense_decode_step
+    out, lse = dense_decode_step(q, c, scale=scale, sliding_window=window, return_lse=True)
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    for b, (k, v) in enumerate(zip(ks, vs)):
+        ref, ref_lse, tol, tol_lse = plain(q[b].cpu(), k, v, scale, window)
+        if len(k) == 0:
+            assert (out[b] == 0).all() and (lse[b] == -math.inf).all()
+            continue
+        seen = v[max(0, len(v) - window):] if window else v
+        tol = tol + (2.0 ** -32 - 2.0 ** -25) * len(seen) * float(seen.abs().max())
+        err = (out[b].double().cpu() - ref).abs()
+        assert (err <= tol).all(), (b, len(k), float((err / tol).max()))
+        assert ((lse[b].double().cpu() - ref_lse).abs() <= tol_lse).all()
+
+
+@pytest.mark.parametrize("paged", [True, False])
+@pytest.mark.parametrize("hq,hkv,dk,dv", [(24, 2, 192, 128), (16, 1, 128, 128), (40, 2, 64, 64), (128, 2, 128, 128), (4, 2, 32, 32)])
+@pytest.mark.parametrize("window", [0, 100])
+def test_float16_at_every_length_within_the_tight_bound(paged, hq, hkv, dk, dv, window):
+    c, ks, vs = make_cache(paged, LENS, 2112, hkv, dk, dv, torch.float16, seed=170)
+    q = randn(len(LENS), hq, dk, seed=171, dtype=torch.float16).to(DEV)
+    check_float16(q, c, ks, vs, window)
+    check_float16(q, c, ks, vs, window, scale=0.4)                 # scores over some 60 powers of two
+
+
+@pytest.mark.parametrize("paged", [True, False])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (192, 128)])
+@pytest.mark.parametrize("lens,cap,hq,hkv", [([1000, 997], 1024, 4, 1), ([2000] * 30, 2048, 8, 4), ([1500] * 20, 2048, 64, 1),
+                                             ([200, 130], 256, 20, 1)])
+def test_float16_far_below_the_maximum_in_every_layout(paged, dk, dv, lens, cap, hq, hkv):
+    """one key with nearly all of the weight and a value of 0, all others at 2^-26.06 of it with values of 1024"""
+    c, ks, vs = make_cache(paged, lens, cap, hkv, dk, dv, torch.float16, seed=180)
+    for k, v in zip(ks, vs):
+        k.zero_()
+        k[0, :, 0] = 4.25
+        v.fill_(1024.0)
+        v[0] = 0.0
+    for b, n in enumerate(lens):
+        for p in range((n + 63) // 64):
+            m, at = min(64, n - 64 * p), slice(64 * p, min(n, 64 * p + 64))
+            k, v = ks[b][at].to(DEV), vs[b][at].permute(1, 2, 0).to(DEV)
+            if paged:
+                page = c.block_table[b, p].long()
+                c.k_pool[page, :m], c.v_pool_t[page, :, :, :m] = k, v
+            else:
+                c.k[b, at], c.vt[b, :, :, at] = k, v
+    q = torch.zeros(len(lens), hq, dk, dtype=torch.float16, device=DEV)
+    q[:, :, 0] = 4.25
+    check_float16(q, c, ks, vs, scale=1.0)
