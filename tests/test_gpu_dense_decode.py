@@ -559,3 +559,41 @@ def test_float16_far_below_the_maximum_in_every_layout(paged, dk, dv, lens, cap,
     q = torch.zeros(len(lens), hq, dk, dtype=torch.float16, device=DEV)
     q[:, :, 0] = 4.25
     check_float16(q, c, ks, vs, scale=1.0)
+
+
+@pytest.mark.parametrize("lens", [[2048] * 33, [2048] * 36, [8192] * 36, [8000] * 38, [4096] * 63, [64 * (130 - b) for b in range(60)],
+                                  [8192] * 34 + [0] * 20, [8192 * 4] + [64] * 62, [640] * 50 + [8192] * 3])
+def test_fewer_sequences_than_units_make_no_second_round(lens):
+    """A workgroup per unit and kv head, one round of them: 1024 of 32 / 32 channels, so 64 units where 16 kv heads share the
+    card.  The partial states in the workspace tell how many units the sequences of more than one were cut into."""
+    from nsa_amd import _lib
+    B, H, D, rows = len(lens), 16, 32, 16
+    cap = (max(lens) + 63) // 64 * 64
+    z = dict(dtype=torch.bfloat16, device=DEV)
+    pages = cap // 64
+    k, v = torch.zeros(pages + 1, 64, H, D, **z), torch.zeros(pages + 1, H, D, 64, **z)
+    k.normal_()
+    v.normal_()
+    table = torch.arange(1, pages + 1, dtype=torch.int32, device=DEV).repeat(B, 1)         # all read the same pages
+    ctx = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    q, out = torch.randn(B, H, D, **z), torch.empty(B, H, D, **z)
+    lib = _lib.load()
+    need = lib.nsa_dense_decode_workspace_bytes(B, H, H, D, D, cap, 0, 0)
+    slots = need // (4 * rows * (D + 2))
+    assert slots == (64 + B) * H
+    ws = torch.full((need // 4,), math.nan, device=DEV)
+    rc = lib.nsa_dense_decode_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), pages, pages + 1, ctx.data_ptr(),
+                                   out.data_ptr(), None, B, H, H, D, D, cap, 0, D ** -0.5, 0, ws.data_ptr(), need,
+                                   torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    written = ~ws[slots * rows * D:].view(slots, rows, 2)[:, 0, 0].isnan()
+    units = int(written.sum()) / H
+    assert units == int(units) and units <= 64
+    for b in range(0, B, 7):                                   # and the result is the sequence's own, however it was cut
+        n = lens[b]
+        if n == 0:
+            assert (out[b] == 0).all()
+            continue
+        kb, vb = k[1:].reshape(-1, H, D)[:n].cpu(), v[1:].permute(0, 3, 1, 2).reshape(-1, H, D)[:n].cpu()
+        ref, _, tol, _ = plain(q[b].cpu(), kb, vb, D ** -0.5, 0)
+        assert ((out[b].double().cpu() - ref).abs() <= tol).all(), b
