@@ -7,7 +7,8 @@
 //
 // Bound by reading K and V once: the matrix instructions of a 32-key chunk take about a tenth of the time its
 // bytes need (128 / 128 channels, 16 heads), so one wavefront simply loads its fragments straight from memory
-// into the operand registers, two chunks ahead of the products, with no LDS in the loop.
+// into the operand registers, with no LDS in the loop: the next chunk's keys are on their way during the softmax and the
+// second product, its values from there on.
 //
 // Work split: a (sequence, kv head) with few others beside it would leave most of the 256 CUs idle, and a ragged
 // batch would wait for its longest sequence.  So the pages of ALL sequences are cut into runs ("units") of the same
@@ -201,7 +202,9 @@ __device__ __forceinline__ void dense_values(DecState<T, DK, DV> (&st)[NT], vec8
 // Registers (32-bit, per lane) of one chunk's fragments, of the queries and sums of NT head tiles, and what else there is.
 template <typename T, int DK, int DV, int NT> constexpr int kDenseRegs =
     (2 * (DK / 32) + DV / 16) * 2 * (int)sizeof(T) + NT * ((DK / 32) * 2 * (int)sizeof(T) + DV / 4) + 48;
-// Wavefronts per SIMD that the register file (512) then holds, of W of a workgroup at least.
+// Wavefronts per SIMD that the register file (512) then holds, of W of a workgroup at least.  The count is short by what a
+// second tile needs besides: 64 / 64 with two tiles and 32 / 32 with four (16-bit) come out at four wavefronts and spill 39
+// to 73 registers, and fp32 192 / 128 at the eight wavefronts of a whole sequence, which need two per SIMD, spills 40.
 template <typename T, int DK, int DV, int NT, int W> constexpr int kDenseOccupancy =
     kDenseRegs<T, DK, DV, NT> <= 128 ? 4 : kDenseRegs<T, DK, DV, NT> <= 168 ? 3 :
     kDenseRegs<T, DK, DV, NT> <= 256 || W > 4 ? 2 : 1;

@@ -3,7 +3,7 @@
 // Pages that end up full are shared by reference count, so a fork copies only what will be written again or lies outside
 // the pages: the partly filled last page and the compressed rows (1/16 of the tokens, contiguous per slot).  The host half
 // (paged_plan) keeps the page table, the counts and the free list, all or nothing, and turns the call into moves in an
-// order in which no slot is overwritten before its readers are done; the device half carries them out in one launch.
+// order in which no slot is overwritten before its readers are done; the device half carries them out, 80 in a launch.
 //
 // Device half: a thread owns the same 16 bytes of every slot (or one column of the page table) and walks over the moves,
 // so even the moves of a permutation need no second buffer: what it has not read yet, nobody has written.  A cycle keeps

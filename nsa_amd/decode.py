@@ -120,7 +120,11 @@ class NSAPagedDecodeCache:
 
     Page bookkeeping (free list, lengths, counts) lives on the host, so no call here waits for the GPU.  If the device half
     of a move fails (a launch error), the host's books no longer fit the device's: the call raises, and so does every later
-    one that would change the cache.  Calls that change a cache are made by one thread and on one stream at a time."""
+    one that would change the cache.
+
+    Calls that change a cache, and nsa_decode_step, which keeps its workspace on it, are made by one thread and on one stream
+    at a time.  dense_decode_step only reads it and has a workspace of its own: such calls may run side by side on several
+    streams, as long as nothing changes the cache meanwhile."""
 
     PAGE = 64
     _lost = False                                        # whether a move's device half failed
@@ -321,7 +325,8 @@ class NSAPagedDecodeCache:
     def fork(self, src: int, dst, length: Optional[int] = None):
         """The sequence of slot src continues in the slots dst (a slot or several) as well, or its first `length` tokens
         do; what dst held is released.  Full pages are shared, the partly filled last page and the compressed rows are
-        copied, in one launch.  RuntimeError, and nothing changes, when the pool has no pages left for the copies."""
+        copied, in one launch per 80 slots.  RuntimeError, and nothing changes, when the pool has no pages left for the
+        copies."""
         dst = [dst] if isinstance(dst, int) else self._ids(dst)
         self._check_slot(src)
         length = self._lens[src] if length is None else length
@@ -543,7 +548,8 @@ def dense_decode_step(q: torch.Tensor, cache, scale: Optional[float] = None, sli
     results over disjoint sets of keys can be joined.  A sequence without tokens yields zeros and -inf.
 
     The tokens of all sequences are cut into equal pieces from the lengths on the device: few long sequences fill the
-    card, a ragged batch does not wait for its longest, and a captured call stays right while the sequences grow.
+    card, a ragged batch does not wait for its longest, and a captured call stays right while the sequences grow.  Infinities
+    and NaN in visible keys and values come out as the formula gives them; the sums exp(s - m) v have to fit fp32.
     out [B,Hq,Dv] / lse float32 [B,Hq]: result buffers of the caller (allocated here when None), which must not overlap
     each other, q or the cache."""
     _need_cuda(q)
