@@ -472,8 +472,8 @@ dense_decode_join_kernel(const DenseDecodeArgs a, int rows_per_slot, int blocks)
 // 16-head tiles that share one pass over the keys: the whole group up to 64 heads (32 in fp32, whose fragments take
 // twice the registers); larger groups read the keys once per block.  Four tiles leave one wavefront per SIMD and join in
 // four rounds, so where there are few pages blocks of two are faster, although both read them (64 / 1 heads of 128 bf16,
-// four tiles against two: 2 sequences of 8192 tokens 20.5 and 15.3 us, 2 of 32768 28.1 and 23.7, 16 of 32768 97 and 103;
-// 192 / 128: 22.1 and 17.4, 30.2 and 29.0, 96 and 148).
+// four tiles against two: 2 sequences of 8192 tokens 20.8 and 14.9 us, 2 of 32768 27.4 and 23.5, 16 of 32768 91 and 94;
+// 192 / 128: 22.4 and 15.9, 29.8 and 25.5, 97 and 115).
 static int dense_tiles(const DenseDecodeArgs& a, long pages) {
   const int G = a.hq / a.hkv;
   if (G <= 16) return 1;
@@ -495,7 +495,7 @@ DensePlan dense_decode_plan(const DenseDecodeArgs& a) {
   const long workgroups = 256 * min(4L, max(1L, 65536 / in_flight));
   // With more sequences than that they come in several rounds anyway; a third of a sequence per unit keeps the last round
   // short (32 / 4 heads of 128 bf16, one unit per sequence against three: 65 sequences of 8192 323 and 247 us, 100 of up
-  // to 8192 252 and 190, 200 of up to 4096 225 and 201; 128 of 4096, which are two rounds to the dot, 200 and 220).
+  // to 8192 213 and 187, 200 of up to 4096 220 and 207; 128 of 4096, which are two rounds to the dot, 200 and 222).
   const long aim = a.batch > workgroups / per ? 3L * a.batch : workgroups / per;
   p.units = (int)max(1L, min(aim, (long)a.batch * span));
   // A short capacity is not worth a second launch: 8 wavefronts take the whole sequence.  16 / 4 heads, split against

@@ -8,9 +8,9 @@
 // Device half: a thread owns the same 16 bytes of every slot (or one column of the page table) and walks over the moves,
 // so even the moves of a permutation need no second buffer: what it has not read yet, nobody has written.  A cycle keeps
 // its first slot's 16 bytes in a register.  Loads of up to 8 moves travel together, and moves that read the same slot
-// share one load.  Bound by HBM: every source is read once, every copy written once (32749 tokens, 4 heads of 128 / 128
-// bf16, into 63 slots: 53 us, 5.2 TB/s; half of 64 slots of 16411 tokens onto the other half: 26 us, 5.5 TB/s), and by the
-// latency of the walk where the slots hold little (a cycle of 16 slots of 4096 tokens: 8.8 us).
+// share one load.  Bound by HBM: every source is read once per group of moves, every copy written once (32749 tokens, 4
+// heads of 128 / 128 bf16, into 63 slots: 53 us, 5.2 TB/s; half of 64 slots of 16411 tokens onto the other half: 26 us,
+// 5.5 TB/s), and by the latency of the walk where the slots hold little (a cycle of 16 slots of 4096 tokens: 8.8 us).
 #include <algorithm>
 #include <vector>
 
