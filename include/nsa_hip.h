@@ -459,7 +459,7 @@ int nsa_decode_step_split_static(const void* q, const void* k_cache, const void*
  * `window` of them, the current one among them.  Cache layouts as above; block_table NULL = contiguous caches (ctx_cap
  * used, a multiple of 64, at most 2^30), else the paged pool of num_pages pages (max_pages used).  The compressed caches are not read.
  *   q [batch][hq][dk]   out [batch][hq][dv]   lse (optional) float [batch][hq]: natural-log log-sum-exp of the scaled scores
- * A sequence with ctx_lens[b] <= 0 yields out = 0 and lse = -inf; a length beyond the capacity counts as the capacity.
+ * A sequence with ctx_lens[b] <= 0, or whose visible scores are all -inf, yields out = 0 and lse = -inf; a length beyond the capacity counts as the capacity.
  * What the cache holds behind a sequence's last token, or before its window, does not matter (not even NaN).  A table
  * entry outside the pool is read as page 0.  Infinities and NaN in visible rows come out as the formula gives them; the
  * sums sum exp(s - m) v are held in fp32 before the division, so they have to fit it.  Any GQA group size; (dk, dv) in (32,32), (64,64), (128,128), (192,128).

@@ -545,7 +545,8 @@ def dense_decode_step(q: torch.Tensor, cache, scale: Optional[float] = None, sli
     `sliding_window` of them when that is positive (the current token, already appended, is one of them).  cache:
     NSADecodeCache or NSAPagedDecodeCache; its compressed rows are not read, so any block / stride will do.  Returns
     out [B,Hq,Dv]; with return_lse also the float32 [B,Hq] natural-log log-sum-exp of the scaled scores, with which
-    results over disjoint sets of keys can be joined.  A sequence without tokens yields zeros and -inf.
+    results over disjoint sets of keys can be joined.  A sequence without tokens, or with no score above -inf, yields zeros
+    and -inf.
 
     The tokens of all sequences are cut into equal pieces from the lengths on the device: few long sequences fill the
     card, a ragged batch does not wait for its longest, and a captured call stays right while the sequences grow.  Infinities

@@ -597,3 +597,29 @@ def test_fewer_sequences_than_units_make_no_second_round(lens):
         kb, vb = k[1:].reshape(-1, H, D)[:n].cpu(), v[1:].permute(0, 3, 1, 2).reshape(-1, H, D)[:n].cpu()
         ref, _, tol, _ = plain(q[b].cpu(), kb, vb, D ** -0.5, 0)
         assert ((out[b].double().cpu() - ref).abs() <= tol).all(), b
+
+
+@pytest.mark.parametrize("cap", [192, 2048])                      # one launch, and the split schedule
+@pytest.mark.parametrize("dtype,group,dk,dv", [(torch.bfloat16, 4, 64, 64), (torch.float16, 20, 128, 128), (torch.float32, 4, 64, 64),
+                                               (torch.bfloat16, 64, 192, 128)])
+def test_infinities_among_the_visible_keys(cap, dtype, group, dk, dv):
+    """a score of -inf takes its key out, one of +inf leaves no number, all of -inf leave nothing: out 0 and lse -inf"""
+    from nsa_amd.decode import dense_decode_step
+    lens = [1, 190, cap, 70]
+    c, ks, vs = make_cache(True, lens, cap, 1, dk, dv, dtype, seed=190)
+    for b, keys in ((0, [0]), (1, [5, 64, 189]), (2, [cap - 1]), (3, range(70))):
+        for j in keys:
+            ks[b][j, 0, 2] = math.inf
+            c.k_pool[c.block_table[b, j // 64].long(), j % 64, 0, 2] = math.inf
+    q = randn(len(lens), group, dk, seed=191, dtype=dtype)
+    q[:, :, 2] = 1.0
+    q[:, ::2, 2] = -1.0
+    out, lse = (t.double().cpu() for t in dense_decode_step(q.to(DEV), c, return_lse=True))
+    for b, n in enumerate(lens):
+        assert out[b, 1::2].isnan().all() and not lse[b, 1::2].isfinite().any(), b
+        if b in (0, 3):
+            assert (out[b, ::2] == 0).all() and (lse[b, ::2] == -math.inf).all()
+            continue
+        seen = ks[b][:, 0, 2].isfinite()
+        ref, ref_lse, tol, tol_lse = plain(q[b, ::2].contiguous(), ks[b][seen], vs[b][seen], dk ** -0.5, 0)
+        assert ((out[b, ::2] - ref).abs() <= tol).all() and ((lse[b, ::2] - ref_lse).abs() <= tol_lse).all(), b
